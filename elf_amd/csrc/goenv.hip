@@ -18,6 +18,7 @@
 #include "../../include/goenv.h"
 #include "goenv_device.h"
 #include "gen_tune.h"
+#include "goenv_host.h"
 #include "goenv_tactics.h"
 
 using namespace goenv;
@@ -1418,45 +1419,6 @@ static int pick_nw_rules(const goenv_ctx* c, int count) {
 // goenv_stats_allreduce)
 constexpr int STATS_ALLOC = GOENV_NUM_STATS + 2;
 
-static thread_local std::string g_err;
-
-static int fail(const char* what, hipError_t e = hipSuccess) {
-  g_err = what;
-  if (e != hipSuccess) {
-    g_err += ": ";
-    g_err += hipGetErrorString(e);
-  }
-  return -1;
-}
-
-#define HIPCHK(x)                                  \
-  do {                                             \
-    hipError_t e_ = (x);                           \
-    if (e_ != hipSuccess) return fail(#x, e_);     \
-  } while (0)
-
-static inline hipStream_t S(void* s) { return (hipStream_t)s; }
-
-// Entry points that launch or copy run with the context's device current and put the caller's
-// device back on return (one host thread may drive several GPUs; a kernel launched on the null
-// stream of another device would be handed pointers that device cannot reach).
-struct DeviceScope {
-  int prev = -1;
-  bool switched = false;
-  hipError_t err;
-  explicit DeviceScope(int dev) {
-    err = hipGetDevice(&prev);
-    if (err == hipSuccess && prev != dev) {
-      err = hipSetDevice(dev);
-      switched = err == hipSuccess;
-    }
-  }
-  ~DeviceScope() {
-    if (switched) (void)hipSetDevice(prev);
-  }
-  DeviceScope(const DeviceScope&) = delete;
-  DeviceScope& operator=(const DeviceScope&) = delete;
-};
 #define ON_DEVICE_OF(c)                       \
   DeviceScope dev_scope_((c)->device);        \
   if (dev_scope_.err != hipSuccess) return fail("selecting the context's device", dev_scope_.err)
