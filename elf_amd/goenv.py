@@ -35,6 +35,35 @@ S_SEQ = 14
 (ST_GAMES, ST_BLACK_WINS, ST_WHITE_WINS, ST_DRAWS, ST_PLIES, ST_BCAP, ST_WCAP, ST_SUM_LEN2, ST_PLY_CAP_HITS,
  ST_MAX_LEN, ST_SUM_SCORE) = range(11)
 
+# Policy-network operators (elf_amd/policy_ops.py): element types, activations, outputs
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
+OUT_KINDS = {"logits": 0, "log_probs": 1, "probs": 2}
+
+
+class Norm(C.Structure):
+    """goenv_norm: the arguments that goenv_group_norm_act and its gradient share."""
+    _fields_ = ([(k, C.c_int32) for k in ("device", "dtype", "param_dtype", "act")] +
+                [("n", C.c_int64), ("positions", C.c_int64), ("channels", C.c_int32), ("groups", C.c_int32),
+                 ("eps", C.c_float), ("slope", C.c_float), ("x", C.c_void_p), ("x_sample", C.c_int64),
+                 ("x_position", C.c_int64), ("residual", C.c_void_p), ("r_sample", C.c_int64),
+                 ("r_position", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p), ("stats", C.c_void_p),
+                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)])
+
+
+class LogitRules(C.Structure):
+    """goenv_logit_rules: the arguments that goenv_policy_logits and its gradient share."""
+    _fields_ = ([(k, C.c_int32) for k in ("device", "dtype", "out_dtype", "out_kind")] +
+                [("rows", C.c_int64), ("cols", C.c_int64), ("logits", C.c_void_p), ("logits_row", C.c_int64),
+                 ("legal", C.c_void_p), ("legal_row", C.c_int64), ("legal_bits", C.c_void_p), ("bits_row", C.c_int64),
+                 ("bias", C.c_void_p), ("bias_row", C.c_int64), ("history", C.c_void_p), ("history_row", C.c_int64),
+                 ("history_len", C.c_void_p), ("history_max", C.c_int32), ("history_i64", C.c_int32),
+                 ("bias_dtype", C.c_int32)] +
+                [(k, C.c_float) for k in ("repetition", "presence", "frequency", "temperature")] +
+                [("row_" + k, C.c_void_p) for k in ("repetition", "presence", "frequency", "temperature")] +
+                [("stats", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)])
+
+
 _lib = None
 
 _SIGS = {
@@ -94,6 +123,14 @@ _SIGS = {
     "goenv_timer_end": (C.c_int, [C.c_void_p, C.c_void_p]),
     "goenv_timer_spin": (C.c_int, [C.c_void_p]),
     "goenv_timer_ms": (C.c_float, [C.c_void_p]),
+    "goenv_group_norm_workspace": (C.c_int64, [C.c_int64, C.c_int64] + [C.c_int] * 4),
+    "goenv_group_norm_act": (C.c_int, [C.POINTER(Norm), C.c_void_p, C.c_void_p]),
+    "goenv_group_norm_act_grad": (C.c_int, [C.POINTER(Norm), C.c_void_p, C.c_int64, C.c_int64] + [C.c_void_p] * 5),
+    "goenv_dropout": (C.c_int, [C.c_int, C.c_int, C.c_int64] + [C.c_void_p] * 3 + [C.c_double, C.c_void_p, C.c_uint32,
+                                C.c_void_p]),
+    "goenv_policy_logits_workspace": (C.c_int64, [C.c_int64, C.c_int64] + [C.c_int] * 3),
+    "goenv_policy_logits": (C.c_int, [C.POINTER(LogitRules), C.c_void_p, C.c_void_p]),
+    "goenv_policy_logits_grad": (C.c_int, [C.POINTER(LogitRules), C.c_void_p, C.c_int64] + [C.c_void_p] * 3),
     "goenv_aug_action": (C.c_int, [C.c_int, C.c_int]),
     "goenv_aug_action_inv": (C.c_int, [C.c_int, C.c_int]),
 }

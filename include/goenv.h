@@ -463,6 +463,129 @@ typedef struct goenv_tactics_out {
 int goenv_tactics(goenv_ctx* ctx, const int32_t* idx, int first, int count, int self_atari_thres,
                   const goenv_tactics_out* out, void* stream);
 
+/* Policy-network operators ---------------------------------------------------
+ * What the network on the other side of a batch needs around its convolutions, from the stem to the
+ * move.  No counterpart in the reference as code of its own (its models are made of torch layers,
+ * go/df_model2.py:28-94); like the rest of the library the calls take device pointers, allocate
+ * nothing, run on `stream` of HIP device `device` and can be captured into a HIP graph.  They need no
+ * context.  A workspace belongs to ONE call in flight: two graphs, or two streams, need one each.
+ * Strides are in elements.  Element types of the arrays: */
+#define GOENV_DT_F32 0
+#define GOENV_DT_BF16 1
+#define GOENV_DT_F16 2
+
+/* goenv_group_norm_act: y = act((x - mean) / sqrt(var + eps) * weight + bias + residual) over
+ * channels-last samples: element (i, p, c) of x at i * x_sample + p * x_position + c.  mean and var
+ * (biased) are taken per sample over all positions and the channels / groups consecutive channels
+ * of a group, held and computed in float32 whatever dtype is.
+ *   residual  NULL, or of x's type with strides of its own
+ *   weight, bias  [channels] of type param_dtype (F32, or dtype), or NULL (1 and 0)
+ *   act       GOENV_ACT_*; slope is the one of LEAKY_RELU
+ *   y         dense [n][positions][channels]
+ *   stats     float32 [n][groups][2], mean and 1 / sqrt(var + eps): what the backward pass needs; NULL if it is not
+ *   workspace at least goenv_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL if that is 0)
+ * Nothing to do (n, positions or channels 0) is no error.
+ * goenv_group_norm_act_grad: the gradients for dy (strides of its own).  z is computed again from x and
+ * residual; with dz = dy * act'(z) and xh the normalised x: dresidual = dz, dbias = sum dz,
+ * dweight = sum dz xh over samples and positions, and dx = rstd (dz w - mean(dz w) - xh mean(dz w xh)),
+ * the means over the group.  dx and dresidual: dense, of type dtype; dweight and dbias: [channels] of type
+ * param_dtype; each may be NULL.  Every sum has a fixed order: equal inputs give equal bits. */
+#define GOENV_ACT_NONE 0
+#define GOENV_ACT_RELU 1
+#define GOENV_ACT_LEAKY_RELU 2
+#define GOENV_ACT_SILU 3
+typedef struct goenv_norm {
+  int32_t device;
+  int32_t dtype, param_dtype;
+  int32_t act;
+  int64_t n, positions;
+  int32_t channels, groups;
+  float eps, slope;
+  const void* x;
+  int64_t x_sample, x_position;
+  const void* residual;
+  int64_t r_sample, r_position;
+  const void* weight;
+  const void* bias;
+  float* stats;
+  void* workspace;
+  uint64_t workspace_bytes;
+} goenv_norm;
+int64_t goenv_group_norm_workspace(int64_t n, int64_t positions, int channels, int groups, int dtype, int grad);
+int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream);
+int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sample, int64_t dy_position, void* dx,
+                              void* dresidual, void* dweight, void* dbias, void* stream);
+
+/* goenv_dropout: y[e] = residual[e] + (keep(e) ? x[e] * 65536 / (65536 - t) : 0) for e in [0, n), with
+ * t = round(p * 65536), 0 <= p <= 1 (t = 65536 drops everything).  The mask is a function of
+ * (seed, step, site, e) and is never stored: the call that is given dy as x and no residual is the
+ * backward pass.  rng: device int64[2] = {seed, step}, read by the kernel -- a captured graph draws a
+ * new mask per replay when `step` is advanced between them; site tells the dropout layers of a step apart.
+ * Elements come in blocks of eight; block b has the 128 bits Philox4x32-10 (Salmon, Moraes, Dror, Shaw:
+ * Parallel random numbers: as easy as 1, 2, 3; 2011) makes of counter (b, b >> 32, step, site) under the key
+ * seed: element j of the block takes the low (j < 4) or high half of word j % 4 and is kept if those 16
+ * bits are >= t.  A dropped element's value is not looked at (a NaN there is dropped too).  y may be x or
+ * residual. */
+int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* residual, void* y, double p,
+                  const int64_t* rng, uint32_t site, void* stream);
+
+/* goenv_policy_logits: from a model's logits to what goenv_sample_policy / goenv_topk_policy take.  Row by row,
+ * with c = how often column v stands in the row's history:
+ *   a = l                                     if c = 0, else
+ *   a = (l > 0 ? l / repetition : l * repetition) - presence - frequency * c
+ *   z = (a + bias) / temperature              -inf where the row's mask forbids v
+ * and out = z (GOENV_OUT_LOGITS), z - log sum exp z (LOG_PROBS) or exp z / sum exp z (PROBS), dense
+ * [rows][cols] of type out_dtype (F32, or dtype); computed in float32.  A column whose z is -inf is off,
+ * whatever made it so; a row with every column off gives -inf, or 0 as probabilities (goenv_sample_policy
+ * then falls back to its uniform policy).  A forbidden column's logit and bias are not looked at.
+ *   legal       u8 [rows][cols], 0 = forbidden (the legal_out of the environment), or NULL
+ *   legal_bits  u32 [rows][(cols + 31) / 32], bit v % 32 of word v / 32 = allowed, or NULL; not both
+ *   bias        of type bias_dtype (F32, or dtype), row stride bias_row (0: one row for all), or NULL
+ *   history     int32, or int64 if history_i64, [rows][history_max]; entries outside [0, cols) (a pass) are
+ *               skipped; history_len int32 [rows], clamped to 0 .. history_max, NULL = history_max
+ *   repetition, presence, frequency, temperature: float32 [rows], or NULL = the scalar of that name.  A row's
+ *               values are used as they are (the scalars must be > 0, finite, finite, > 0).
+ *   stats       float32 [rows][2], the row's largest z and sum exp(z - largest): for the backward pass of
+ *               LOG_PROBS and PROBS; else NULL
+ *   workspace   at least goenv_policy_logits_workspace(..., 0) bytes, 16-byte aligned (NULL if that is 0)
+ * goenv_policy_logits_grad: dlogits (dense, of type dtype) and dbias (of type bias_dtype; [cols] if bias_row
+ * is 0, else dense [rows][cols]) for d_out of type out_dtype, row stride dy_row; either may be NULL.
+ * Columns that are off have no gradient and pass none on: what d_out holds there is not looked at.  The
+ * penalties and the temperature have none. */
+#define GOENV_OUT_LOGITS 0
+#define GOENV_OUT_LOG_PROBS 1
+#define GOENV_OUT_PROBS 2
+typedef struct goenv_logit_rules {
+  int32_t device;
+  int32_t dtype, out_dtype, out_kind;
+  int64_t rows, cols;
+  const void* logits;
+  int64_t logits_row;
+  const uint8_t* legal;
+  int64_t legal_row;
+  const uint32_t* legal_bits;
+  int64_t bits_row;
+  const void* bias;
+  int64_t bias_row;
+  const void* history;
+  int64_t history_row;
+  const int32_t* history_len;
+  int32_t history_max, history_i64;
+  int32_t bias_dtype;
+  float repetition, presence, frequency, temperature;
+  const float* row_repetition;
+  const float* row_presence;
+  const float* row_frequency;
+  const float* row_temperature;
+  float* stats;
+  void* workspace;
+  uint64_t workspace_bytes;
+} goenv_logit_rules;
+int64_t goenv_policy_logits_workspace(int64_t rows, int64_t cols, int out_kind, int shared_bias, int grad);
+int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream);
+int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int64_t dy_row, void* dlogits, void* dbias,
+                             void* stream);
+
 /* Statistics ---------------------------------------------------------------
  * goenv_finish: score every finished board that has not been counted yet and
  * add it to the device stats vector (boards keep their state).
