@@ -59,22 +59,477 @@ __device__ __forceinline__ float block_max(float v, float* lds) {
 }
 
 // ---- group norm ---------------------------------------------------------------------------------
+//
+// y = act((x - mean) rstd w + b + residual) per sample and group.  Bound by memory: the forward pass has to read x and the residual
+// and write y once (2,048 boards of 128 bf16 channels: 568 MB, 117 us = 4.9 TB/s, what a copy of that size reaches), the
+// backward pass reads x, dy and the residual and writes dx and dresidual (256 boards: 118 MB, 26 us and 3 us for the channels' sums).
+// So a sample's slab of a few groups is held by one workgroup, in LDS, from the first read to the write: the mean and then the
+// squared deviations about it (not sums of squares, which lose the variance of data far from zero) are taken from LDS.  The loads
+// go to LDS directly, without registers in between: with the slab in registers a thread's loads waited for each other
+// and occupancy was three waves a SIMD (159 us for the case above).
 
-__device__ __forceinline__ float act_of(int act, float slope, float z) {
-  if (act == GOENV_ACT_SILU) return z / (1.f + __expf(-z));
-  if (z > 0.f) return z;
-  return slope == 0.f ? (z != z ? z : 0.f) : z * slope;
+// The hardware's exponential and reciprocal are off by about one step of float32 each; a division in full costs ten
+// instructions an element.
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+// y = act(z), and dz = dy * act'(z).  (A NaN stays one; -inf and an infinite dy on the flat side of relu give 0.)
+template <int ACT>
+__device__ __forceinline__ float act_of(float slope, float z) {
+  if (ACT == GOENV_ACT_RELU) return z <= 0.f ? 0.f : z;
+  if (ACT == GOENV_ACT_LEAKY_RELU) return z > 0.f ? z : z * slope;
+  if (ACT == GOENV_ACT_SILU) return z * sigmoid(z);
+  return z;
 }
-__device__ __forceinline__ float act_grad(int act, float slope, float z) {
-  if (act == GOENV_ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return s * (1.f + z * (1.f - s));
+template <int ACT>
+__device__ __forceinline__ float act_grad(float slope, float z, float dy) {
+  if (ACT == GOENV_ACT_RELU) return z <= 0.f ? 0.f : dy;
+  if (ACT == GOENV_ACT_LEAKY_RELU) return z > 0.f ? dy : dy * slope;
+  if (ACT == GOENV_ACT_SILU) {
+    const float s = sigmoid(z);
+    return dy * (s * (1.f + z * (1.f - s)));
   }
-  return z > 0.f ? 1.f : slope;
+  return dy;
+}
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+// f(activation as a constant): the choice is made once, around a loop
+template <typename F>
+__host__ __device__ __forceinline__ void by_act(int act, F f) {
+  if (act == GOENV_ACT_RELU) f(Int<GOENV_ACT_RELU>());
+  else if (act == GOENV_ACT_LEAKY_RELU) f(Int<GOENV_ACT_LEAKY_RELU>());
+  else if (act == GOENV_ACT_SILU) f(Int<GOENV_ACT_SILU>());
+  else f(Int<GOENV_ACT_NONE>());
+}
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// `VEC` channels' weights or biases
+template <int VEC>
+__device__ __forceinline__ void load_params(const void* p, int dt, int c, float missing, float (&to)[VEC]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) to[j] = missing;
+  } else if (dt == GOENV_DT_F32) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) to[j] = static_cast<const float*>(p)[c + j];
+  } else if (dt == GOENV_DT_BF16) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) to[j] = (float)static_cast<const __bf16*>(p)[c + j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) to[j] = (float)static_cast<const _Float16*>(p)[c + j];
+  }
+}
+
+// How a launch cuts the work: a workgroup has one sample's slab of slab_groups whole groups (width channels, units vectors of
+// VEC channels a position) and the positions of one chunk; its threads are rows x units.
+struct NormCut {
+  int slab_groups, width, units, rows, slabs, chunks;
+  int staged, scratch;    // vectors of a thread that are staged in LDS (of each array), behind this many floats of scratch
+  int64_t chunk;          // positions of a chunk (the last one may have fewer)
+};
+
+constexpr int NORM_THREADS = 512;   // the most that a workgroup has
+
+enum NormPhase { NORM_WHOLE, NORM_SUMS, NORM_APPLY };
+
+// This thread's place in a launch: `count` positions of the chunk, from `first` on, `rows` apart.
+struct NormPlace {
+  int64_t sample, first, chunk_size;
+  int c0, unit, row, part, count;   // first channel of the slab; the vector of the position; the row; the chunk
+  bool on;                          // the thread has a row
+};
+__device__ __forceinline__ NormPlace norm_place(const goenv_norm& P, const NormCut& cut) {
+  NormPlace q;
+  // Workgroups go to the eight XCDs in turn; each XCD takes a run of neighbours, so that what lies next to each other in memory (the
+  // slabs of a sample share cache lines) meets in one L2.
+  const uint32_t xcd = blockIdx.x & 7, share = gridDim.x >> 3, over = gridDim.x & 7;
+  uint32_t b = xcd * share + (xcd < over ? xcd : over) + (blockIdx.x >> 3);
+  q.part = (int)(b % (uint32_t)cut.chunks);
+  b /= (uint32_t)cut.chunks;
+  q.c0 = (int)(b % (uint32_t)cut.slabs) * cut.width;
+  q.sample = b / (uint32_t)cut.slabs;
+  const int64_t lo = q.part * cut.chunk;
+  q.chunk_size = lo + cut.chunk < P.positions ? cut.chunk : P.positions - lo;
+  q.unit = threadIdx.x % cut.units;
+  q.row = threadIdx.x / cut.units;
+  q.on = q.row < cut.rows;
+  q.first = lo + (q.on && q.row < q.chunk_size ? q.row : 0);   // an address inside the sample for every thread
+  q.count = q.on && q.row < q.chunk_size ? ((int)q.chunk_size - q.row + cut.rows - 1) / cut.rows : 0;
+  return q;
+}
+
+__device__ __forceinline__ bool is_pow2(int v) { return (v & (v - 1)) == 0; }
+
+// Sums over a slab's groups.  Each thread brings its vector's sum: NV = 1 where a vector lies within one group, else a value per
+// channel.  Where the vectors of a position and of a group are powers of two that fit a wave, lanes are added up by
+// exchanges and a group's sum is one value per wave; elsewhere a wave adds up a group's values from LDS.  Returned
+// for the thread's channels (group_of(j) of its own).  lds: threads * NV + groups floats; every thread of the workgroup calls.
+template <int VEC, int NV>
+__device__ __forceinline__ void slab_sum(const NormCut& cut, int cpg, const NormPlace& q, float (&val)[NV], float* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  if (!q.on)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) val[j] = 0.f;
+  const int per = NV == 1 ? cpg / VEC : 0;   // vectors of a group
+  if (NV == 1 && cut.units <= 64 && is_pow2(cut.units) && is_pow2(per)) {
+    float v = val[0];
+    for (int d = 1; d < per; d <<= 1) v += __shfl_xor(v, d);
+    for (int d = cut.units; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    const int g = q.unit / per;
+    if (lane < cut.units && q.unit % per == 0) lds[wave * cut.slab_groups + g] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int w = 0; w < waves; ++w) v += lds[w * cut.slab_groups + g];
+    val[0] = v;
+    __syncthreads();
+    return;
+  }
+  float* total = lds + blockDim.x * NV;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) lds[threadIdx.x * NV + j] = val[j];
+  __syncthreads();
+  const int mine = NV == 1 ? per : cpg;     // a group's values per row: they lie next to each other
+  for (int g = wave; g < cut.slab_groups; g += waves) {
+    float v = 0.f;
+    for (int k = lane; k < cut.rows * mine; k += 64) {
+      const int row = k / mine;
+      v += lds[row * cut.units * NV + g * mine + (k - row * mine)];
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    if (lane == 0) total[g] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NV; ++j) val[j] = total[NV == 1 ? q.unit / per : (q.unit * VEC + j) / cpg];
+  __syncthreads();
+}
+
+// Arrays that are read through LDS: a thread's slot k of an area is its own, what it puts there only it reads.  Vectors of 16 bytes go
+// there without passing through registers (a wave's 64 slots lie next to each other, as the instruction wants them), so that
+// all of a thread's loads are under way at once.
+template <typename T, int VEC>
+__device__ __forceinline__ void stage(const T* from, Pack<T, VEC>* area, int k) {
+  if constexpr (sizeof(Pack<T, VEC>) == 16) {
+    Pack<T, VEC>* wave0 = area + k * blockDim.x + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)wave0, 16, 0, 0);
+  } else {
+    area[k * blockDim.x + threadIdx.x] = load_pack<T, VEC>(from);
+  }
+}
+
+// Before the first read of a staged slot: the loads to LDS are counted with the loads from memory, and nothing else waits for them.
+__device__ __forceinline__ void staged_here() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> staged_pack(const Pack<T, VEC>* slot) {
+  if constexpr (sizeof(Pack<T, VEC>) == 16) {
+    typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(Pack<T, VEC>, *reinterpret_cast<const Quad*>(slot));   // one 16-byte read
+  } else {
+    return *slot;
+  }
+}
+
+// Group norm of a slab's chunk.  x and the residual are read once, into LDS (the first `staged` vectors of a thread; what does not fit
+// is read again in each pass, from the caches).  WHOLE: statistics, normalisation, residual and activation in one
+// launch.  SUMS: a chunk's mean and sum of squared deviations to the workspace [n][groups][chunks].  APPLY: joins the chunks' and
+// applies them.
+template <typename T, int VEC, bool ONE, bool RES, int PHASE>
+__global__ __launch_bounds__(NORM_THREADS) void k_group_norm(goenv_norm P, NormCut cut, T* y) {
+  extern __shared__ __align__(16) float lds[];
+  constexpr int NV = ONE ? 1 : VEC;
+  const int cpg = P.channels / P.groups;
+  const NormPlace q = norm_place(P, cut);
+  const int c = q.c0 + q.unit * VEC;
+  const T* x = static_cast<const T*>(P.x) + q.sample * P.x_sample + q.first * P.x_position + c;
+  const T* r = RES ? static_cast<const T*>(P.residual) + q.sample * P.r_sample + q.first * P.r_position + c : nullptr;
+  const int64_t xs = cut.rows * P.x_position, rs = cut.rows * P.r_position, os = (int64_t)cut.rows * P.channels;
+  Pack<T, VEC>*area = reinterpret_cast<Pack<T, VEC>*>(lds + cut.scratch), *area2 = area + cut.staged * blockDim.x;
+  const int staged = q.count < cut.staged ? q.count : cut.staged;
+  for (int k = 0; k < staged; ++k) stage<T, VEC>(x + k * xs, area, k);
+  if (RES)
+    for (int k = 0; k < staged; ++k) stage<T, VEC>(r + k * rs, area2, k);
+  float w[VEC], b[VEC];
+  load_params<VEC>(P.weight, P.param_dtype, c, 1.f, w);
+  load_params<VEC>(P.bias, P.param_dtype, c, 0.f, b);
+  staged_here();
+
+  float mean[NV], rstd[NV];
+  if (PHASE != NORM_APPLY) {
+    const float inv_m = 1.f / ((float)q.chunk_size * (float)cpg);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) mean[j] = rstd[j] = 0.f;
+    auto add = [&](const Pack<T, VEC>& a) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) mean[ONE ? 0 : j] += (float)a.v[j];
+    };
+    for (int k = 0; k < staged; ++k) add(staged_pack(&area[k * blockDim.x + threadIdx.x]));
+    for (int k = staged; k < q.count; ++k) add(load_pack<T, VEC>(x + k * xs));
+    slab_sum<VEC, NV>(cut, cpg, q, mean, lds);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) mean[j] *= inv_m;
+    auto square = [&](const Pack<T, VEC>& a) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = (float)a.v[j] - mean[ONE ? 0 : j];
+        rstd[ONE ? 0 : j] += d * d;
+      }
+    };
+    for (int k = 0; k < staged; ++k) square(staged_pack(&area[k * blockDim.x + threadIdx.x]));
+    for (int k = staged; k < q.count; ++k) square(load_pack<T, VEC>(x + k * xs));
+    slab_sum<VEC, NV>(cut, cpg, q, rstd, lds);
+    if (PHASE == NORM_WHOLE)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) rstd[j] = 1.f / sqrtf(rstd[j] * inv_m + P.eps);
+    // one thread per group says what it has
+    float2* to = PHASE == NORM_SUMS ? static_cast<float2*>(P.workspace) : reinterpret_cast<float2*>(P.stats);
+    if (to && q.on && q.row == 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if ((c + j) % cpg == 0) to[(q.sample * P.groups + (c + j) / cpg) * cut.chunks + q.part] = make_float2(mean[j], rstd[j]);
+    }
+    if (PHASE == NORM_SUMS) return;
+  } else {
+    // mean = sum n_k mean_k / n; the deviations about it: sum of M2_k + n_k (mean_k - mean)^2
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int g = wave; g < cut.slab_groups; g += waves) {
+      const int64_t at = q.sample * P.groups + q.c0 / cpg + g;
+      const float2* part = static_cast<const float2*>(P.workspace) + at * cut.chunks;
+      const float inv_m = 1.f / ((float)P.positions * (float)cpg);
+      auto size = [&](int k) { return (float)((k + 1) * cut.chunk < P.positions ? cut.chunk : P.positions - k * cut.chunk) * (float)cpg; };
+      float m = 0.f, s = 0.f;
+      for (int k = lane; k < cut.chunks; k += 64) m += size(k) * part[k].x;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) m += __shfl_xor(m, d);
+      m *= inv_m;
+      for (int k = lane; k < cut.chunks; k += 64) {
+        const float2 v = part[k];
+        s += v.y + size(k) * (v.x - m) * (v.x - m);
+      }
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+      s = 1.f / sqrtf(s * inv_m + P.eps);
+      if (lane == 0) {
+        lds[2 * g] = m;
+        lds[2 * g + 1] = s;
+        if (P.stats && q.part == 0) reinterpret_cast<float2*>(P.stats)[at] = make_float2(m, s);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int g = (q.unit * VEC + j) / cpg;
+      mean[j] = lds[2 * g];
+      rstd[j] = lds[2 * g + 1];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) w[j] *= rstd[ONE ? 0 : j];
+  T* o = y + (q.sample * P.positions + q.first) * P.channels + c;
+  by_act(P.act, [&](auto act) {
+    auto apply = [&](int k, const Pack<T, VEC>& a, const Pack<T, VEC>& e) {
+      Pack<T, VEC> out;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float z = ((float)a.v[j] - mean[ONE ? 0 : j]) * w[j] + b[j];
+        if (RES) z += (float)e.v[j];
+        out.v[j] = (T)act_of<decltype(act)::value>(P.slope, z);
+      }
+      *reinterpret_cast<Pack<T, VEC>*>(o + k * os) = out;
+    };
+    for (int k = 0; k < staged; ++k) {
+      const int at = k * blockDim.x + threadIdx.x;
+      apply(k, staged_pack(&area[at]), RES ? staged_pack(&area2[at]) : Pack<T, VEC>());
+    }
+    for (int k = staged; k < q.count; ++k) apply(k, load_pack<T, VEC>(x + k * xs), RES ? load_pack<T, VEC>(r + k * rs) : Pack<T, VEC>());
+  });
+}
+
+// The gradients of a slab's chunk, cut and staged as above.  WHOLE: the channels' sums of dz and dz xh (to the workspace,
+// [n][chunks][channels], for k_group_norm_param_grad), the groups' means from them, dx and dresidual.  SUMS: the sums alone.
+// APPLY: joins the chunks' sums; dx and dresidual.
+template <typename T, int VEC, bool RES, int PHASE>
+__global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, NormCut cut, const T* dy0, int64_t dy_sample,
+                                                                  int64_t dy_position, T* dx, T* dr) {
+  extern __shared__ __align__(16) float lds[];
+  const int cpg = P.channels / P.groups, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const NormPlace q = norm_place(P, cut);
+  const int c = q.c0 + q.unit * VEC;
+  const T* x = static_cast<const T*>(P.x) + q.sample * P.x_sample + q.first * P.x_position + c;
+  const T* r = RES ? static_cast<const T*>(P.residual) + q.sample * P.r_sample + q.first * P.r_position + c : nullptr;
+  const T* dy = dy0 + q.sample * dy_sample + q.first * dy_position + c;
+  const int64_t xs = cut.rows * P.x_position, rs = cut.rows * P.r_position, gs = cut.rows * dy_position, os = (int64_t)cut.rows * P.channels;
+  Pack<T, VEC>*area = reinterpret_cast<Pack<T, VEC>*>(lds + cut.scratch), *area2 = area + cut.staged * blockDim.x,
+             *area3 = area2 + cut.staged * blockDim.x;
+  const int staged = q.count < cut.staged ? q.count : cut.staged;
+  for (int k = 0; k < staged; ++k) {
+    stage<T, VEC>(x + k * xs, area, k);
+    stage<T, VEC>(dy + k * gs, area2, k);
+    if (RES) stage<T, VEC>(r + k * rs, area3, k);
+  }
+  float w[VEC], b[VEC], mean[VEC], rstd[VEC];
+  load_params<VEC>(P.weight, P.param_dtype, c, 1.f, w);
+  load_params<VEC>(P.bias, P.param_dtype, c, 0.f, b);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const float2 st = reinterpret_cast<const float2*>(P.stats)[q.sample * P.groups + (c + j) / cpg];
+    mean[j] = st.x;
+    rstd[j] = st.y;
+  }
+  staged_here();
+  // f(j, xh, dz) for every element of the thread's
+  auto each = [&](auto f, auto done) {
+    by_act(P.act, [&](auto act) {
+      auto one = [&](int k, const Pack<T, VEC>& a, const Pack<T, VEC>& g, const Pack<T, VEC>& e) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float xh = ((float)a.v[j] - mean[j]) * rstd[j];
+          float z = xh * w[j] + b[j];
+          if (RES) z += (float)e.v[j];
+          f(j, xh, act_grad<decltype(act)::value>(P.slope, z, (float)g.v[j]));
+        }
+        done(k);
+      };
+      for (int k = 0; k < staged; ++k) {
+        const int at = k * blockDim.x + threadIdx.x;
+        one(k, staged_pack(&area[at]), staged_pack(&area2[at]), RES ? staged_pack(&area3[at]) : Pack<T, VEC>());
+      }
+      for (int k = staged; k < q.count; ++k)
+        one(k, load_pack<T, VEC>(x + k * xs), load_pack<T, VEC>(dy + k * gs), RES ? load_pack<T, VEC>(r + k * rs) : Pack<T, VEC>());
+    });
+  };
+  float2* part = static_cast<float2*>(P.workspace);
+  float* sum1 = lds;                       // [width] of w dz, then of w dz xh: a channel's
+  float* sum2 = lds + cut.width;
+  float* group = sum2 + cut.width;         // [slab_groups][2]: a group's means
+  float* red = group + 2 * cut.slab_groups;
+  if (PHASE != NORM_APPLY) {
+    float a1[VEC], a2[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a1[j] = a2[j] = 0.f;
+    each(
+        [&](int j, float xh, float dz) {
+          a1[j] += dz;
+          a2[j] += dz * xh;
+        },
+        [](int) {});
+    // over the rows: by exchanges where the units of a position are a power of two that fits a wave, then over the waves (or all rows)
+    const bool pow2 = cut.units <= 64 && is_pow2(cut.units);
+    if (pow2)
+      for (int d = cut.units; d < 64; d <<= 1)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          a1[j] += __shfl_xor(a1[j], d);
+          a2[j] += __shfl_xor(a2[j], d);
+        }
+    const int from = pow2 ? wave : q.row, many = pow2 ? waves : cut.rows;
+    if (pow2 ? lane < cut.units : q.on)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        red[(from * 2) * cut.width + q.unit * VEC + j] = a1[j];
+        red[(from * 2 + 1) * cut.width + q.unit * VEC + j] = a2[j];
+      }
+    __syncthreads();
+    for (int k = threadIdx.x; k < cut.width; k += blockDim.x) {
+      float s1 = 0.f, s2 = 0.f;
+      for (int i = 0; i < many; ++i) {
+        s1 += red[(i * 2) * cut.width + k];
+        s2 += red[(i * 2 + 1) * cut.width + k];
+      }
+      part[(q.sample * cut.chunks + q.part) * P.channels + q.c0 + k] = make_float2(s1, s2);
+      const float wk = P.weight ? load_any(P.weight, P.param_dtype, q.c0 + k) : 1.f;
+      sum1[k] = wk * s1;
+      sum2[k] = wk * s2;
+    }
+    if (PHASE == NORM_SUMS) return;
+  } else {
+    for (int k = threadIdx.x; k < cut.width; k += blockDim.x) {
+      float s1 = 0.f, s2 = 0.f;
+      for (int i = 0; i < cut.chunks; ++i) {
+        const float2 v = part[(q.sample * cut.chunks + i) * P.channels + q.c0 + k];
+        s1 += v.x;
+        s2 += v.y;
+      }
+      const float wk = P.weight ? load_any(P.weight, P.param_dtype, q.c0 + k) : 1.f;
+      sum1[k] = wk * s1;
+      sum2[k] = wk * s2;
+    }
+  }
+  __syncthreads();
+  for (int g = wave; g < cut.slab_groups; g += waves) {
+    float m1 = 0.f, m2 = 0.f;
+    for (int k = lane; k < cpg; k += 64) {
+      m1 += sum1[g * cpg + k];
+      m2 += sum2[g * cpg + k];
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      m1 += __shfl_xor(m1, d);
+      m2 += __shfl_xor(m2, d);
+    }
+    const float inv_m = 1.f / ((float)P.positions * (float)cpg);
+    if (lane == 0) {
+      group[2 * g] = m1 * inv_m;
+      group[2 * g + 1] = m2 * inv_m;
+    }
+  }
+  __syncthreads();
+  float m1[VEC], m2[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const int g = (q.unit * VEC + j) / cpg;
+    m1[j] = group[2 * g];
+    m2[j] = group[2 * g + 1];
+  }
+  const int64_t o = (q.sample * P.positions + q.first) * P.channels + c;
+  Pack<T, VEC> ox, orr;
+  each(
+      [&](int j, float xh, float dz) {
+        orr.v[j] = (T)dz;
+        ox.v[j] = (T)(rstd[j] * (dz * w[j] - m1[j] - xh * m2[j]));
+      },
+      [&](int k) {
+        if (dx) *reinterpret_cast<Pack<T, VEC>*>(dx + o + k * os) = ox;
+        if (dr) *reinterpret_cast<Pack<T, VEC>*>(dr + o + k * os) = orr;
+      });
+}
+
+// dbias and dweight: the sums of the samples' (and chunks') parts, 16 channels (a cache line) a workgroup, 64 rows at a time
+__global__ __launch_bounds__(1024) void k_group_norm_param_grad(const float2* part, int64_t rows, int channels, int param_dtype, void* dweight,
+                                                                void* dbias) {
+  __shared__ float2 lds[64][16];
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+  float a = 0.f, b = 0.f;
+  if (c < channels)
+#pragma unroll 4
+    for (int64_t i = row; i < rows; i += 64) {
+      const float2 v = part[i * channels + c];
+      a += v.x;
+      b += v.y;
+    }
+  lds[row][col] = make_float2(a, b);
+  __syncthreads();
+  if (row != 0 || c >= channels) return;
+  for (int i = 1; i < 64; ++i) {
+    a += lds[i][col].x;
+    b += lds[i][col].y;
+  }
+  if (dbias) store_any(dbias, param_dtype, c, a);
+  if (dweight) store_any(dweight, param_dtype, c, b);
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_group_norm(goenv_norm P, T* y) {
+__global__ __launch_bounds__(256) void k_group_norm_any(goenv_norm P, T* y) {
   __shared__ float lds[4];
   const int cpg = P.channels / P.groups;
   const int64_t m = P.positions * cpg;
@@ -104,14 +559,14 @@ __global__ __launch_bounds__(256) void k_group_norm(goenv_norm P, T* y) {
       if (P.weight) z *= load_any(P.weight, P.param_dtype, c0 + c);
       if (P.bias) z += load_any(P.bias, P.param_dtype, c0 + c);
       if (r) z += (float)r[p * P.r_position + c];
-      o[p * P.channels + c] = (T)act_of(P.act, P.slope, z);
+      by_act(P.act, [&](auto a) { o[p * P.channels + c] = (T)act_of<decltype(a)::value>(P.slope, z); });
     }
   }
 }
 
 // dx and dresidual of one sample's group, and its channels' part of dbias and dweight into workspace [n][channels][2]
 template <typename T>
-__global__ __launch_bounds__(256) void k_group_norm_grad(goenv_norm P, const T* dy0, int64_t dy_sample, int64_t dy_position, T* dx0,
+__global__ __launch_bounds__(256) void k_group_norm_any_grad(goenv_norm P, const T* dy0, int64_t dy_sample, int64_t dy_position, T* dx0,
                                                          T* dr0) {
   __shared__ float lds[4];
   const int cpg = P.channels / P.groups;
@@ -133,7 +588,8 @@ __global__ __launch_bounds__(256) void k_group_norm_grad(goenv_norm P, const T* 
         const float xh = ((float)x[p * P.x_position + c] - mean) * rstd;
         float z = xh * w + b;
         if (r) z += (float)r[p * P.r_position + c];
-        const float dz = (float)dy[p * dy_position + c] * act_grad(P.act, P.slope, z);
+        float dz;
+        by_act(P.act, [&](auto a) { dz = act_grad<decltype(a)::value>(P.slope, z, (float)dy[p * dy_position + c]); });
         a1 += dz;
         a2 += dz * xh;
       }
@@ -152,25 +608,12 @@ __global__ __launch_bounds__(256) void k_group_norm_grad(goenv_norm P, const T* 
       const float xh = ((float)x[p * P.x_position + c] - mean) * rstd;
       float z = xh * w + b;
       if (r) z += (float)r[p * P.r_position + c];
-      const float dz = (float)dy[p * dy_position + c] * act_grad(P.act, P.slope, z);
+      float dz;
+      by_act(P.act, [&](auto a) { dz = act_grad<decltype(a)::value>(P.slope, z, (float)dy[p * dy_position + c]); });
       if (dr0) dr0[o] = (T)dz;
       if (dx0) dx0[o] = (T)(rstd * (dz * w - m1 - xh * m2));
     }
   }
-}
-
-__global__ __launch_bounds__(256) void k_group_norm_param_grad(const float2* part, int64_t rows, int channels, int param_dtype, void* dweight,
-                                                               void* dbias) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= channels) return;
-  float a = 0.f, b = 0.f;
-  for (int64_t i = 0; i < rows; ++i) {
-    const float2 v = part[i * channels + c];
-    a += v.x;
-    b += v.y;
-  }
-  if (dbias) store_any(dbias, param_dtype, c, a);
-  if (dweight) store_any(dweight, param_dtype, c, b);
 }
 
 // ---- dropout ------------------------------------------------------------------------------------
@@ -372,12 +815,110 @@ void by_dtype(int dt, F f) {
   else f(_Float16());
 }
 
+
+// ---- host: group norm ---------------------------------------------------------------------------
+
+// The widest vector that divides a row of channels
+int norm_vec(int channels, int dtype) {
+  const int most = dtype == GOENV_DT_F32 ? 4 : 8;
+  if (channels % most == 0) return most;
+  return dtype != GOENV_DT_F32 && channels % 2 == 0 ? 2 : 1;
+}
+
+struct NormPlan {
+  NormCut cut;
+  int threads, vec;
+  size_t lds;      // bytes of the staging launches
+  bool split;
+};
+
+// `vec` 0: the widest vector; else what the arrays' alignment allows (the cut into slabs and chunks stays the same)
+NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int dtype, bool residual, bool grad, int vec = 0) {
+  NormPlan p;
+  const int cpg = channels / groups, widest = norm_vec(channels, dtype), size = dtype == GOENV_DT_F32 ? 4 : 2;
+  // Slabs: as narrow as whole groups and vectors allow, but 64 bytes of a position where that leaves 512 workgroups (2,048 boards
+  // of 128 bf16 channels in 8 groups: 32 bytes 150 us, 64 bytes 123 us, 128 bytes 134 us).
+  auto next_of = [&](int gs) {
+    do ++gs;
+    while (gs <= groups && (groups % gs || (gs * cpg) % widest));
+    return gs;
+  };
+  int gs = next_of(0);
+  while (gs < groups && gs * cpg * size < 64 && n * (groups / next_of(gs)) >= 512) gs = next_of(gs);
+  // Threads: few vectors each while there are few workgroups, six where there are many.
+  auto vectors_at = [&](int threads, int64_t of) {
+    const int rows = threads / (gs * cpg / widest);
+    return rows ? (of + rows - 1) / rows : of;
+  };
+  auto threads_for = [&](int64_t of, int most) {
+    int t = 64;
+    while (t < NORM_THREADS && (t < gs * cpg / widest || vectors_at(t, of) > most)) t *= 2;
+    return t;
+  };
+  const int64_t wgs = n * (groups / gs);
+  p.threads = threads_for(positions, wgs < 64 ? 2 : wgs < 512 ? 3 : 6);
+  // A long axis with few workgroups is cut into chunks of `part` vectors a thread, at most `many`.
+  int64_t chunks = 1;
+  const int part = grad ? 8 : 4, many = grad ? 32 : 64;
+  if (wgs < 256 && vectors_at(NORM_THREADS, positions) > 12) {
+    while (gs < groups && gs * cpg * size < (grad ? 64 : 128)) gs = next_of(gs);
+    p.threads = NORM_THREADS;
+    chunks = (vectors_at(p.threads, positions) + part - 1) / part;
+    if (chunks > many) chunks = many;
+  }
+  const int most = (grad ? 32 : 48) << 10;
+  NormCut& c = p.cut;
+  p.vec = vec ? vec : widest;
+  c.slab_groups = gs;
+  c.width = gs * cpg;
+  c.slabs = groups / gs;
+  c.chunk = (positions + chunks - 1) / chunks;
+  c.chunks = (int)((positions + c.chunk - 1) / c.chunk);
+  c.units = c.width / p.vec;
+  c.rows = p.threads / c.units;
+  p.split = c.chunks > 1;
+  if (c.rows == 0) return p;
+  if (grad) {
+    const int parts = c.units <= 64 && (c.units & (c.units - 1)) == 0 ? p.threads / 64 : c.rows;
+    c.scratch = 2 * c.width + 2 * gs + 2 * parts * c.width;
+  } else {
+    c.scratch = p.threads * (cpg % p.vec == 0 ? 1 : p.vec) + 2 * gs;
+  }
+  c.scratch = (c.scratch + 3) & ~3;
+  const int64_t vectors = (c.chunk + c.rows - 1) / c.rows, row = (int64_t)p.threads * p.vec * size * (1 + grad + residual);
+  c.staged = (int)(vectors < most / row ? vectors : most / row);
+  p.lds = c.scratch * sizeof(float) + c.staged * row;
+  return p;
+}
+
+// The widest vector that the arrays' alignment allows
+int norm_fit(const goenv_norm* a, const void* dy, int64_t dy_sample, int64_t dy_position, const void* o1, const void* o2) {
+  const int size = a->dtype == GOENV_DT_F32 ? 4 : 2, vec = norm_vec(a->channels, a->dtype);
+  auto fits = [&](int v) {
+    int64_t all = (int64_t)(uintptr_t)a->x | (int64_t)(uintptr_t)a->residual | (int64_t)(uintptr_t)dy | (int64_t)(uintptr_t)o1 | (int64_t)(uintptr_t)o2;
+    all |= (a->x_sample | a->x_position | dy_sample | dy_position) * size;
+    if (a->residual) all |= (a->r_sample | a->r_position) * size;
+    return (all & (v * size - 1)) == 0;
+  };
+  return fits(vec) ? vec : vec > 2 && size == 2 && fits(2) ? 2 : 1;
+}
+
+// f(vector width)
+template <typename T, typename F>
+void by_vec(int vec, F f) {
+  if (vec == 1) return f(Int<1>());
+  if constexpr (sizeof(T) == 2)
+    if (vec == 2) return f(Int<2>());
+  f(Int<16 / sizeof(T)>());
+}
+
 int check_norm(const goenv_norm* p, bool grad) {
   if (!p) return fail("goenv_group_norm_act: p is NULL");
   if (!is_dtype(p->dtype)) return fail("goenv_group_norm_act: dtype must be GOENV_DT_F32, BF16 or F16");
   if (p->param_dtype != GOENV_DT_F32 && p->param_dtype != p->dtype)
     return fail("goenv_group_norm_act: param_dtype must be GOENV_DT_F32 or dtype");
   if (p->n < 0 || p->positions < 0 || p->channels < 0) return fail("goenv_group_norm_act: a size is negative");
+  if (p->positions > INT32_MAX) return fail("goenv_group_norm_act: more than 2^31 - 1 positions");
   if (p->groups <= 0 || p->channels % p->groups) return fail("goenv_group_norm_act: groups must divide channels");
   if (p->act < GOENV_ACT_NONE || p->act > GOENV_ACT_SILU) return fail("goenv_group_norm_act: act must be a GOENV_ACT_*");
   if (!(p->eps >= 0.f) || isinf(p->eps)) return fail("goenv_group_norm_act: eps must be finite and not negative");
@@ -393,10 +934,9 @@ int check_norm(const goenv_norm* p, bool grad) {
     return fail("goenv_group_norm_act: the workspace is too small or not 16-byte aligned (goenv_group_norm_workspace)");
   return 0;
 }
-goenv_norm with_slope(const goenv_norm* p) {
+goenv_norm with_act(const goenv_norm* p) {
   goenv_norm q = *p;
-  if (q.act == GOENV_ACT_NONE) q.slope = 1.f;
-  if (q.act == GOENV_ACT_RELU) q.slope = 0.f;
+  if (q.act == GOENV_ACT_LEAKY_RELU && q.slope == 0.f) q.act = GOENV_ACT_RELU;
   return q;
 }
 
@@ -437,8 +977,10 @@ int check_logits(const goenv_logit_rules* p, bool grad) {
 extern "C" {
 
 int64_t goenv_group_norm_workspace(int64_t n, int64_t positions, int channels, int groups, int dtype, int grad) {
-  (void)positions, (void)groups, (void)dtype;
-  return grad ? n * channels * (int64_t)sizeof(float2) : 0;
+  if (n <= 0 || positions <= 0 || channels <= 0 || groups <= 0 || channels % groups) return 0;
+  const NormPlan plan = norm_plan(n, positions, channels, groups, dtype, true, grad);
+  if (grad) return n * plan.cut.chunks * channels * (int64_t)sizeof(float2);
+  return plan.split ? n * plan.cut.chunks * groups * (int64_t)sizeof(float2) : 0;
 }
 
 int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream) {
@@ -446,10 +988,31 @@ int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream) {
   if (p->n == 0 || p->positions == 0 || p->channels == 0) return 0;
   if (!y || !aligned(y, p->dtype)) return fail("goenv_group_norm_act: y is required, aligned to its elements");
   ON_DEVICE(p->device, "goenv_group_norm_act");
-  const goenv_norm q = with_slope(p);
+  const goenv_norm q = with_act(p);
+  const NormPlan plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, false, norm_fit(&q, nullptr, 0, 0, y, nullptr));
   by_dtype(p->dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_group_norm<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<T*>(y));
+    if (plan.cut.rows == 0) {
+      hipLaunchKernelGGL((k_group_norm_any<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<T*>(y));
+      return;
+    }
+    by_vec<T>(plan.vec, [&](auto v) {
+      constexpr int VEC = decltype(v)::value;
+      const dim3 grid((unsigned)(q.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
+      const bool one = (q.channels / q.groups) % VEC == 0;
+      auto go = [&](auto f) { hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), q, plan.cut, static_cast<T*>(y)); };
+      auto with = [&](auto o, auto r) {
+        constexpr bool ONE = decltype(o)::value, RES = decltype(r)::value;
+        if (!plan.split) {
+          go(k_group_norm<T, VEC, ONE, RES, NORM_WHOLE>);
+        } else {
+          go(k_group_norm<T, VEC, ONE, false, NORM_SUMS>);
+          go(k_group_norm<T, VEC, ONE, RES, NORM_APPLY>);
+        }
+      };
+      if (one) q.residual ? with(Int<1>(), Int<1>()) : with(Int<1>(), Int<0>());
+      else q.residual ? with(Int<0>(), Int<1>()) : with(Int<0>(), Int<0>());
+    });
   });
   HIPCHK(hipGetLastError());
   return 0;
@@ -463,18 +1026,42 @@ int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sa
   if (!empty && (!dy || !aligned(dy, p->dtype) || !aligned(dx, p->dtype) || !aligned(dresidual, p->dtype)))
     return fail("goenv_group_norm_act_grad: dy is required, and the arrays aligned to their elements");
   ON_DEVICE(p->device, "goenv_group_norm_act_grad");
-  const goenv_norm q = with_slope(p);
+  const goenv_norm q = with_act(p);
+  NormPlan plan = {};
   if (!empty) {
+    plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, true, norm_fit(&q, dy, dy_sample, dy_position, dx, dresidual));
     by_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
-      hipLaunchKernelGGL((k_group_norm_grad<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<const T*>(dy),
-                         dy_sample, dy_position, static_cast<T*>(dx), static_cast<T*>(dresidual));
+      if (plan.cut.rows == 0) {
+        plan.cut.chunks = 1;
+        hipLaunchKernelGGL((k_group_norm_any_grad<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<const T*>(dy),
+                           dy_sample, dy_position, static_cast<T*>(dx), static_cast<T*>(dresidual));
+        return;
+      }
+      by_vec<T>(plan.vec, [&](auto v) {
+        constexpr int VEC = decltype(v)::value;
+        const dim3 grid((unsigned)(q.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
+        auto go = [&](auto f) {
+          hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), q, plan.cut, static_cast<const T*>(dy), dy_sample, dy_position,
+                             static_cast<T*>(dx), static_cast<T*>(dresidual));
+        };
+        auto with = [&](auto r) {
+          constexpr bool RES = decltype(r)::value;
+          if (!plan.split) {
+            go(k_group_norm_grad<T, VEC, RES, NORM_WHOLE>);
+          } else {
+            go(k_group_norm_grad<T, VEC, RES, NORM_SUMS>);
+            if (dx || dresidual) go(k_group_norm_grad<T, VEC, RES, NORM_APPLY>);
+          }
+        };
+        q.residual ? with(Int<1>()) : with(Int<0>());
+      });
     });
     HIPCHK(hipGetLastError());
   }
   if (dweight || dbias) {
-    hipLaunchKernelGGL(k_group_norm_param_grad, dim3((q.channels + 255) / 256), dim3(256), 0, S(stream),
-                       static_cast<const float2*>(q.workspace), empty ? 0 : q.n, q.channels, q.param_dtype, dweight, dbias);
+    hipLaunchKernelGGL(k_group_norm_param_grad, dim3((q.channels + 15) / 16), dim3(1024), 0, S(stream),
+                       static_cast<const float2*>(q.workspace), empty ? 0 : q.n * plan.cut.chunks, q.channels, q.param_dtype, dweight, dbias);
     HIPCHK(hipGetLastError());
   }
   return 0;
