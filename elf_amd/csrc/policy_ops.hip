@@ -656,8 +656,18 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t n, const T* x, const T*
 }
 
 // ---- policy logits ------------------------------------------------------------------------------
+//
+// A row's columns are cut into slices of threads x NI vectors of VEC columns, one workgroup each, with the slice's columns
+// in registers; how often a column stands in the row's history is counted in LDS (integers: the order does not matter).  Bound by
+// memory for many rows or long ones, by latency for a short one; so a row that fits one slice takes one launch and reads everything
+// once.  Longer rows take a launch for the slices' maxima and sums and one that joins them and computes z again, which costs
+// reading the logits a second time (from the caches) instead of writing and reading z in 32 bits.
 
-constexpr int LOGIT_CHUNK = 4096;   // columns whose history counts are in LDS at a time
+struct LogitCut {
+  int slices, per_group;   // slices of a row; rows that one workgroup takes one after the other
+  int64_t groups;          // of rows
+};
+enum LogitMode { LOGIT_MAP, LOGIT_WHOLE, LOGIT_SUMS, LOGIT_APPLY };   // no softmax; softmax in one launch, or in two
 
 struct RowRules {
   float inv_rep, rep, presence, frequency, inv_t;
@@ -671,130 +681,297 @@ __device__ __forceinline__ RowRules rules_of(const goenv_logit_rules& P, int64_t
   r.inv_t = 1.f / (P.row_temperature ? P.row_temperature[row] : P.temperature);
   return r;
 }
-__device__ __forceinline__ bool allowed(const goenv_logit_rules& P, int64_t row, int64_t v) {
-  if (P.legal) return P.legal[row * P.legal_row + v] != 0;
-  if (P.legal_bits) return (P.legal_bits[row * P.bits_row + (v >> 5)] >> (v & 31)) & 1u;
-  return true;
-}
-// z of a column, and dz / dlogit without the temperature in `slope`
-template <typename T>
-__device__ __forceinline__ float z_of(const goenv_logit_rules& P, const RowRules& r, int64_t row, int64_t v, int count, float& slope) {
-  slope = 1.f;
-  if (!allowed(P, row, v)) return -INFINITY;
-  float a = (float)static_cast<const T*>(P.logits)[row * P.logits_row + v];
-  if (count > 0) {
-    slope = a > 0.f ? r.inv_rep : r.rep;
-    a = a * slope - r.presence - r.frequency * (float)count;
+
+// NI vectors of an array of type F32 or T.  The columns behind the last vector read that one again.
+template <typename T, int VEC, int NI>
+__device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at, const int (&col)[NI], float (&to)[NI][VEC]) {
+  if (f32) {
+    Pack<float, VEC> v[NI];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) v[k] = load_pack<float, VEC>(static_cast<const float*>(p) + at + col[k]);
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) to[k][j] = v[k].v[j];
+  } else {
+    Pack<T, VEC> v[NI];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) v[k] = load_pack<T, VEC>(static_cast<const T*>(p) + at + col[k]);
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) to[k][j] = (float)v[k].v[j];
   }
-  if (P.bias) a += load_any(P.bias, P.bias_dtype, row * P.bias_row + v);
-  return a * r.inv_t;
 }
-// counts of columns [v0, v0 + LOGIT_CHUNK) in the row's history
-__device__ __forceinline__ void count_chunk(const goenv_logit_rules& P, int64_t row, int64_t v0, int* count) {
-  __syncthreads();
-  for (int k = threadIdx.x; k < LOGIT_CHUNK; k += 256) count[k] = 0;
-  __syncthreads();
+template <typename T, int VEC, int NI>
+__device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, const int (&col)[NI], const bool (&in)[NI], const float (&from)[NI][VEC]) {
+  if (f32) {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      Pack<float, VEC> v;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v.v[j] = from[k][j];
+      if (in[k]) *reinterpret_cast<Pack<float, VEC>*>(static_cast<float*>(p) + at + col[k]) = v;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      Pack<T, VEC> v;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v.v[j] = (T)from[k][j];
+      if (in[k]) *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(p) + at + col[k]) = v;
+    }
+  }
+}
+
+// This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end), and dz / dlogit without the
+// temperature.  count: LDS, a word per column of the slice; every thread of the workgroup calls.
+template <typename T, int VEC, int NI>
+__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const RowRules& r, int64_t row, int v0, const int (&col)[NI],
+                                         const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
+  load_columns<T, VEC, NI>(P.logits, sizeof(T) == 4, row * P.logits_row, col, z);
+  uint32_t mask[NI];
+  if (P.legal) {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const uint8_t* at = P.legal + row * P.legal_row + col[k];
+      if constexpr (VEC == 4) mask[k] = *reinterpret_cast<const uint32_t*>(at);
+      else mask[k] = *at;
+    }
+  } else if (P.legal_bits) {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) mask[k] = P.legal_bits[row * P.bits_row + (col[k] >> 5)];
+  }
+  float bias[NI][VEC];
+  if (P.bias) load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, row * P.bias_row, col, bias);
   if (P.history) {
+    __syncthreads();   // the row before has read its counts
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) count[(k * blockDim.x + threadIdx.x) * VEC + j] = 0;
+    __syncthreads();
     int len = P.history_len ? P.history_len[row] : P.history_max;
     len = len < 0 ? 0 : len > P.history_max ? P.history_max : len;
-    for (int k = threadIdx.x; k < len; k += 256) {
-      const int64_t at = row * P.history_row + k;
-      const int64_t v = P.history_i64 ? static_cast<const int64_t*>(P.history)[at] : static_cast<const int32_t*>(P.history)[at];
-      if (v >= v0 && v < v0 + LOGIT_CHUNK && v < P.cols) atomicAdd(&count[v - v0], 1);
+    const int width = NI * VEC * blockDim.x;
+    auto mark = [&](int64_t v) {
+      const int64_t at = v - v0;
+      if (at >= 0 && at < width && v < P.cols) atomicAdd(&count[at], 1);
+    };
+    if (P.history_i64) {
+      const int64_t* h = static_cast<const int64_t*>(P.history) + row * P.history_row;
+      for (int k = threadIdx.x; k < len; k += blockDim.x) mark(h[k]);
+    } else {
+      const int32_t* h = static_cast<const int32_t*>(P.history) + row * P.history_row;
+      for (int k = threadIdx.x; k < len; k += blockDim.x) mark(h[k]);
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int c = count[(k * blockDim.x + threadIdx.x) * VEC + j];
+        const float l = z[k][j], f = l > 0.f ? r.inv_rep : r.rep;
+        slope[k][j] = c > 0 ? f : 1.f;
+        z[k][j] = c > 0 ? l * f - r.presence - r.frequency * (float)c : l;
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) slope[k][j] = 1.f;
   }
-  __syncthreads();
+  if (P.bias)
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) z[k][j] += bias[k][j];
+  const bool bytes = P.legal != nullptr, masked = bytes || P.legal_bits != nullptr;
+#pragma unroll
+  for (int k = 0; k < NI; ++k)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const uint32_t m = bytes ? mask[k] & (0xffu << (8 * j)) : mask[k] & (1u << ((col[k] + j) & 31));
+      z[k][j] = (masked && m == 0) || !in[k] ? -INFINITY : z[k][j] * r.inv_t;
+    }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_policy_logits(goenv_logit_rules P, void* out) {
-  __shared__ int count[LOGIT_CHUNK];
-  __shared__ float lds[4];
-  for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
-    const RowRules r = rules_of(P, row);
-    float m = -INFINITY, s = 0.f, slope;
-    if (P.out_kind != GOENV_OUT_LOGITS) {
-      for (int64_t v0 = 0; v0 < P.cols; v0 += LOGIT_CHUNK) {
-        count_chunk(P, row, v0, count);
-        for (int64_t v = v0 + threadIdx.x; v < P.cols && v < v0 + LOGIT_CHUNK; v += 256) {
-          const float z = z_of<T>(P, r, row, v, count[v - v0], slope);
-          if (z == -INFINITY) continue;
-          const float top = fmaxf(m, z);
-          s = s * (m == -INFINITY ? 0.f : expf(m - top)) + expf(z - top);
-          m = top;
-        }
-      }
-      const float top = block_max<4>(m, lds);
-      s = block_sum<4>(m == -INFINITY ? s : s * expf(m - top), lds);
-      m = top == -INFINITY ? 0.f : top;
-      if (P.stats && threadIdx.x == 0) {
-        P.stats[2 * row] = m;
-        P.stats[2 * row + 1] = s;
-      }
+// Over a workgroup of any number of waves, the same order every time.  lds: 16 floats.
+template <typename F>
+__device__ __forceinline__ float block_join(float v, float* lds, F f) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = f(v, __shfl_xor(v, d));
+  const int waves = blockDim.x >> 6;
+  if (waves == 1) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
+  for (int w = 1; w < waves; ++w) v = f(v, lds[w]);
+  return v;
+}
+__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
+
+template <int VEC, int NI>
+__device__ __forceinline__ void columns_of(const goenv_logit_rules& P, int v0, int (&col)[NI], bool (&in)[NI]) {
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    const int64_t v = v0 + (int64_t)(k * blockDim.x + threadIdx.x) * VEC;
+    in[k] = v < P.cols;
+    col[k] = in[k] ? (int)v : (int)P.cols - VEC;
+  }
+}
+
+// The workspace of the two launches: a row's slices' (largest z, sum exp(z - largest)).
+template <typename T, int VEC, int NI, int MODE>
+__global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, LogitCut cut, void* out) {
+  extern __shared__ __align__(16) int count[];
+  __shared__ float lds[16];
+  const int64_t row = blockIdx.x / (uint32_t)cut.slices;
+  const int slice = (int)(blockIdx.x % (uint32_t)cut.slices), v0 = slice * NI * VEC * (int)blockDim.x;
+  int col[NI];
+  bool in[NI];
+  columns_of<VEC, NI>(P, v0, col, in);
+  float z[NI][VEC], slope[NI][VEC];
+  slice_of<T, VEC, NI>(P, rules_of(P, row), row, v0, col, in, count, z, slope);
+  if (MODE != LOGIT_MAP) {
+    float m = -INFINITY, s = 0.f;
+    if (MODE != LOGIT_APPLY) {
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = fmaxf(m, z[k][j]);
+      m = block_join(m, lds, fmaxf);
+      if (m == -INFINITY) m = 0.f;    // nothing left: every exponential is 0
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += __expf(z[k][j] - m);
+      s = block_join(s, lds, add_f);
+    }
+    float2* part = static_cast<float2*>(P.workspace) + row * cut.slices;
+    if (MODE == LOGIT_SUMS) {
+      if (threadIdx.x == 0) part[slice] = make_float2(s == 0.f ? -INFINITY : m, s);
+      return;
+    }
+    if (MODE == LOGIT_APPLY) {
+      // every wave joins the slices by itself
+      const int lane = threadIdx.x & 63;
+      for (int k = lane; k < cut.slices; k += 64) m = fmaxf(m, part[k].x);
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+      if (m == -INFINITY) m = 0.f;
+      for (int k = lane; k < cut.slices; k += 64) s += part[k].y == 0.f ? 0.f : part[k].y * __expf(part[k].x - m);
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+    }
+    if (P.stats && slice == 0 && threadIdx.x == 0) {
+      P.stats[2 * row] = m;
+      P.stats[2 * row + 1] = s;
     }
     const float log_s = logf(s), inv_s = 1.f / s;
-    for (int64_t v0 = 0; v0 < P.cols; v0 += LOGIT_CHUNK) {
-      count_chunk(P, row, v0, count);
-      for (int64_t v = v0 + threadIdx.x; v < P.cols && v < v0 + LOGIT_CHUNK; v += 256) {
-        const float z = z_of<T>(P, r, row, v, count[v - v0], slope);
-        float o = z;
-        if (P.out_kind == GOENV_OUT_PROBS) o = z == -INFINITY ? 0.f : expf(z - m) * inv_s;
-        if (P.out_kind == GOENV_OUT_LOG_PROBS) o = z == -INFINITY ? z : z - m - log_s;
-        store_any(out, P.out_dtype, row * P.cols + v, o);
+    const bool probs = P.out_kind == GOENV_OUT_PROBS;
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = z[k][j] - m;
+        z[k][j] = z[k][j] == -INFINITY ? (probs ? 0.f : -INFINITY) : probs ? __expf(d) * inv_s : d - log_s;
       }
-    }
   }
+  store_columns<T, VEC, NI>(out, P.out_dtype == GOENV_DT_F32, row * P.cols, col, in, z);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_policy_logits_grad(goenv_logit_rules P, const void* d_out, int64_t dy_row, T* dlogits, void* dbias,
-                                                            float* dz_out) {
-  __shared__ int count[LOGIT_CHUNK];
-  __shared__ float lds[4];
-  for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
+// The gradients.  The workspace: a row's slices' sums of dy (log probabilities) or p dy (probabilities), then the row groups'
+// sums of dz for a bias that all rows share.
+template <typename T, int VEC, int NI, int MODE>
+__global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P, LogitCut cut, const void* d_out, int64_t dy_row, T* dlogits,
+                                                             void* dbias, float* shared) {
+  extern __shared__ __align__(16) int count[];
+  __shared__ float lds[16];
+  const int64_t group = blockIdx.x / (uint32_t)cut.slices;
+  const int slice = (int)(blockIdx.x % (uint32_t)cut.slices), v0 = slice * NI * VEC * (int)blockDim.x;
+  int col[NI];
+  bool in[NI];
+  columns_of<VEC, NI>(P, v0, col, in);
+  float sum[NI][VEC];
+#pragma unroll
+  for (int k = 0; k < NI; ++k)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[k][j] = 0.f;
+  const int64_t end = (group + 1) * cut.per_group < P.rows ? (group + 1) * cut.per_group : P.rows;
+  for (int64_t row = group * cut.per_group; row < end; ++row) {
     const RowRules r = rules_of(P, row);
-    float total = 0.f, m = 0.f, inv_s = 0.f, slope;
-    if (P.out_kind != GOENV_OUT_LOGITS) {
-      m = P.stats[2 * row];
-      inv_s = 1.f / P.stats[2 * row + 1];
-      for (int64_t v0 = 0; v0 < P.cols; v0 += LOGIT_CHUNK) {
-        count_chunk(P, row, v0, count);
-        for (int64_t v = v0 + threadIdx.x; v < P.cols && v < v0 + LOGIT_CHUNK; v += 256) {
-          const float z = z_of<T>(P, r, row, v, count[v - v0], slope);
-          if (z == -INFINITY) continue;
-          const float dy = load_any(d_out, P.out_dtype, row * dy_row + v);
-          total += P.out_kind == GOENV_OUT_PROBS ? dy * expf(z - m) * inv_s : dy;
+    float z[NI][VEC], slope[NI][VEC], dz[NI][VEC];
+    load_columns<T, VEC, NI>(d_out, P.out_dtype == GOENV_DT_F32, row * dy_row, col, dz);
+    slice_of<T, VEC, NI>(P, r, row, v0, col, in, count, z, slope);
+    if (MODE != LOGIT_MAP) {
+      const float m = P.stats[2 * row], inv_s = 1.f / P.stats[2 * row + 1];
+      const bool probs = P.out_kind == GOENV_OUT_PROBS;
+      float total = 0.f;
+      float* part = static_cast<float*>(P.workspace) + row * cut.slices;
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const bool off = z[k][j] == -INFINITY;
+          const float p = __expf(z[k][j] - m) * inv_s;
+          slope[k][j] = off ? 0.f : slope[k][j];
+          dz[k][j] = off ? 0.f : dz[k][j];
+          z[k][j] = off ? 0.f : p;
+          total += probs ? z[k][j] * dz[k][j] : dz[k][j];
         }
+      if (MODE == LOGIT_APPLY) {
+        total = 0.f;
+        for (int k = threadIdx.x & 63; k < cut.slices; k += 64) total += part[k];
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+      } else {
+        total = block_join(total, lds, add_f);
       }
-      total = block_sum<4>(total, lds);
+      if (MODE == LOGIT_SUMS) {
+        if (threadIdx.x == 0) part[slice] = total;
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dz[k][j] = probs ? z[k][j] * (dz[k][j] - total) : dz[k][j] - z[k][j] * total;
     }
-    for (int64_t v0 = 0; v0 < P.cols; v0 += LOGIT_CHUNK) {
-      count_chunk(P, row, v0, count);
-      for (int64_t v = v0 + threadIdx.x; v < P.cols && v < v0 + LOGIT_CHUNK; v += 256) {
-        const float z = z_of<T>(P, r, row, v, count[v - v0], slope);
-        float dz = 0.f;
-        if (z != -INFINITY) {
-          dz = load_any(d_out, P.out_dtype, row * dy_row + v);
-          if (P.out_kind == GOENV_OUT_PROBS) dz = expf(z - m) * inv_s * (dz - total);
-          if (P.out_kind == GOENV_OUT_LOG_PROBS) dz -= expf(z - m) * inv_s * total;
-          dz *= r.inv_t;
-        } else {
-          slope = 0.f;
-        }
-        if (dlogits) dlogits[row * P.cols + v] = (T)(z == -INFINITY ? 0.f : dz * slope);
-        if (dz_out) dz_out[row * P.cols + v] = dz;
-        else if (dbias) store_any(dbias, P.bias_dtype, row * P.cols + v, dz);
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (MODE == LOGIT_MAP && z[k][j] == -INFINITY) dz[k][j] = slope[k][j] = 0.f;
+        dz[k][j] *= r.inv_t;
+        sum[k][j] += dz[k][j];
       }
+    if (dbias && !shared) store_columns<T, VEC, NI>(dbias, P.bias_dtype == GOENV_DT_F32, row * P.cols, col, in, dz);
+    if (dlogits) {
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dz[k][j] *= slope[k][j];
+      store_columns<T, VEC, NI>(dlogits, sizeof(T) == 4, row * P.cols, col, in, dz);
     }
   }
+  if (MODE != LOGIT_SUMS && shared) store_columns<float, VEC, NI>(shared, true, group * P.cols, col, in, sum);
 }
 
-__global__ __launch_bounds__(256) void k_column_sum(const float* part, int64_t rows, int64_t cols, int dtype, void* out) {
-  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < cols; v += (int64_t)gridDim.x * 256) {
-    float a = 0.f;
-    for (int64_t i = 0; i < rows; ++i) a += part[i * cols + v];
-    store_any(out, dtype, v, a);
-  }
+// Column sums of [rows][cols], 16 columns (half a cache line) a workgroup, 64 rows at a time
+__global__ __launch_bounds__(1024) void k_column_sum(const float* part, int64_t rows, int64_t cols, int dtype, void* out) {
+  __shared__ float lds[64][16];
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t v = (int64_t)blockIdx.x * 16 + col;
+  float a = 0.f;
+  if (v < cols)
+#pragma unroll 4
+    for (int64_t i = row; i < rows; i += 64) a += part[i * cols + v];
+  lds[row][col] = a;
+  __syncthreads();
+  if (row != 0 || v >= cols) return;
+  for (int i = 1; i < 64; ++i) a += lds[i][col];
+  store_any(out, dtype, v, a);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -912,6 +1089,45 @@ void by_vec(int vec, F f) {
   f(Int<16 / sizeof(T)>());
 }
 
+// ---- host: policy logits --------------------------------------------------------------------------
+
+struct LogitPlan {
+  LogitCut cut;
+  int threads, vec, ni;
+  bool split;
+};
+
+// The cut for vectors of `vec` columns (which goes by the arrays' alignment: a workspace is sized for either).  The gradient holds four
+// values a column, twice what the forward pass holds.
+LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, bool grad, int vec) {
+  LogitPlan p;
+  p.vec = vec;
+  p.ni = vec == 1 ? 6 : grad ? 2 : 4;
+  const int each = p.ni * vec;             // columns of a thread
+  p.split = softmax && cols > 1024 * each;
+  p.threads = 64;
+  while (p.threads < (p.split || !softmax ? 256 : 1024) && (int64_t)p.threads * each < cols) p.threads *= 2;
+  p.cut.slices = (int)((cols + (int64_t)p.threads * each - 1) / ((int64_t)p.threads * each));
+  p.cut.per_group = 1;
+  if (shared) {
+    const int64_t wgs = rows * p.cut.slices, most = rows < 65536 ? rows : 65536;
+    p.cut.per_group = (int)(wgs <= 1024 ? 1 : (wgs + 1023) / 1024 < most ? (wgs + 1023) / 1024 : most);
+  }
+  p.cut.groups = (rows + p.cut.per_group - 1) / p.cut.per_group;
+  return p;
+}
+
+// Whether all arrays allow vectors of four columns
+bool logit_fours(const goenv_logit_rules* p, const void* d_out, int64_t dy_row, const void* o1, int o1_dtype, const void* o2, int o2_dtype) {
+  auto fits = [](const void* a, int dt, int64_t row) {
+    const int64_t size = dt == GOENV_DT_F32 ? 4 : 2;
+    return a == nullptr || ((((int64_t)(uintptr_t)a) | (row * size)) & (4 * size - 1)) == 0;
+  };
+  return p->cols % 4 == 0 && fits(p->logits, p->dtype, p->logits_row) && fits(p->bias, p->bias_dtype, p->bias_row) &&
+         fits(d_out, p->out_dtype, dy_row) && fits(o1, o1_dtype, p->cols) && fits(o2, o2_dtype, p->cols) &&
+         (p->legal == nullptr || (((uintptr_t)p->legal | (uintptr_t)p->legal_row) & 3) == 0);
+}
+
 int check_norm(const goenv_norm* p, bool grad) {
   if (!p) return fail("goenv_group_norm_act: p is NULL");
   if (!is_dtype(p->dtype)) return fail("goenv_group_norm_act: dtype must be GOENV_DT_F32, BF16 or F16");
@@ -990,6 +1206,7 @@ int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream) {
   ON_DEVICE(p->device, "goenv_group_norm_act");
   const goenv_norm q = with_act(p);
   const NormPlan plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, false, norm_fit(&q, nullptr, 0, 0, y, nullptr));
+  if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks) return fail("goenv_group_norm_act: too many samples for one launch");
   by_dtype(p->dtype, [&](auto t) {
     using T = decltype(t);
     if (plan.cut.rows == 0) {
@@ -1030,6 +1247,8 @@ int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sa
   NormPlan plan = {};
   if (!empty) {
     plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, true, norm_fit(&q, dy, dy_sample, dy_position, dx, dresidual));
+    if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks)
+      return fail("goenv_group_norm_act_grad: too many samples for one launch");
     by_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
       if (plan.cut.rows == 0) {
@@ -1089,18 +1308,44 @@ int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* r
 }
 
 int64_t goenv_policy_logits_workspace(int64_t rows, int64_t cols, int out_kind, int shared_bias, int grad) {
-  (void)out_kind;
-  return grad && shared_bias ? rows * cols * (int64_t)sizeof(float) : 0;
+  if (rows <= 0 || cols <= 0) return 0;
+  const bool softmax = out_kind != GOENV_OUT_LOGITS;
+  int64_t most = 0;
+  for (int vec : {1, 4}) {
+    const LogitPlan p = logit_plan(rows, cols, softmax, grad && shared_bias, grad, vec);
+    int64_t need = p.split ? rows * p.cut.slices * (int64_t)(grad ? sizeof(float) : sizeof(float2)) : 0;
+    if (grad && shared_bias) need = ((need + 15) & ~15) + p.cut.groups * cols * (int64_t)sizeof(float);
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream) {
   if (check_logits(p, false)) return -1;
   if (p->rows == 0 || p->cols == 0) return 0;
   if (!out || !aligned(out, p->out_dtype)) return fail("goenv_policy_logits: out is required, aligned to its elements");
+  const bool softmax = p->out_kind != GOENV_OUT_LOGITS;
+  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, false, false, logit_fours(p, nullptr, 0, out, p->out_dtype, nullptr, 0) ? 4 : 1);
+  if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits");
   by_dtype(p->dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_policy_logits<T>), dim3(grid_of(p->rows)), dim3(256), 0, S(stream), *p, out);
+    auto with = [&](auto v, auto n) {
+      constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
+      const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
+      auto go = [&](auto f) {
+        hipLaunchKernelGGL(f, dim3((unsigned)(p->rows * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, out);
+      };
+      if (!softmax) {
+        go(k_policy_logits<T, VEC, NI, LOGIT_MAP>);
+      } else if (!plan.split) {
+        go(k_policy_logits<T, VEC, NI, LOGIT_WHOLE>);
+      } else {
+        go(k_policy_logits<T, VEC, NI, LOGIT_SUMS>);
+        go(k_policy_logits<T, VEC, NI, LOGIT_APPLY>);
+      }
+    };
+    plan.vec == 4 ? with(Int<4>(), Int<4>()) : with(Int<1>(), Int<6>());
   });
   HIPCHK(hipGetLastError());
   return 0;
@@ -1110,21 +1355,41 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
   if (check_logits(p, true)) return -1;
   if (dbias && !p->bias) return fail("goenv_policy_logits_grad: dbias without a bias");
   if (p->cols == 0) return 0;
-  const bool shared = dbias && p->bias_row == 0;
+  const bool shared = dbias && p->bias_row == 0, softmax = p->out_kind != GOENV_OUT_LOGITS;
   if (p->rows > 0 && (!d_out || !aligned(d_out, p->out_dtype) || !aligned(dlogits, p->dtype) || !aligned(dbias, p->bias_dtype)))
     return fail("goenv_policy_logits_grad: d_out is required, and the arrays aligned to their elements");
+  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, shared, true,
+                                    logit_fours(p, d_out, dy_row, dlogits, p->dtype, shared ? nullptr : dbias, p->bias_dtype) ? 4 : 1);
+  if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits_grad: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits_grad");
+  const int64_t sums = plan.split ? (p->rows * plan.cut.slices * (int64_t)sizeof(float) + 15) & ~15 : 0;
+  float* parts = shared ? reinterpret_cast<float*>(static_cast<char*>(p->workspace) + sums) : nullptr;
   if (p->rows > 0) {
     by_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
-      hipLaunchKernelGGL((k_policy_logits_grad<T>), dim3(grid_of(p->rows)), dim3(256), 0, S(stream), *p, d_out, dy_row,
-                         static_cast<T*>(dlogits), dbias, shared ? static_cast<float*>(p->workspace) : nullptr);
+      auto with = [&](auto v, auto n) {
+        constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
+        const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
+        auto go = [&](auto f) {
+          hipLaunchKernelGGL(f, dim3((unsigned)(plan.cut.groups * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, d_out,
+                             dy_row, static_cast<T*>(dlogits), dbias, parts);
+        };
+        if (!softmax) {
+          go(k_policy_logits_grad<T, VEC, NI, LOGIT_MAP>);
+        } else if (!plan.split) {
+          go(k_policy_logits_grad<T, VEC, NI, LOGIT_WHOLE>);
+        } else {
+          go(k_policy_logits_grad<T, VEC, NI, LOGIT_SUMS>);
+          go(k_policy_logits_grad<T, VEC, NI, LOGIT_APPLY>);
+        }
+      };
+      plan.vec == 4 ? with(Int<4>(), Int<2>()) : with(Int<1>(), Int<6>());
     });
     HIPCHK(hipGetLastError());
   }
   if (shared) {
-    hipLaunchKernelGGL(k_column_sum, dim3(grid_of((p->cols + 255) / 256)), dim3(256), 0, S(stream), static_cast<const float*>(p->workspace),
-                       p->rows, p->cols, p->bias_dtype, dbias);
+    hipLaunchKernelGGL(k_column_sum, dim3((unsigned)((p->cols + 15) / 16)), dim3(1024), 0, S(stream), parts, p->rows > 0 ? plan.cut.groups : 0,
+                       p->cols, p->bias_dtype, dbias);
     HIPCHK(hipGetLastError());
   }
   return 0;
