@@ -35,12 +35,7 @@ S_SEQ = 14
 (ST_GAMES, ST_BLACK_WINS, ST_WHITE_WINS, ST_DRAWS, ST_PLIES, ST_BCAP, ST_WCAP, ST_SUM_LEN2, ST_PLY_CAP_HITS,
  ST_MAX_LEN, ST_SUM_SCORE) = range(11)
 
-# Policy-network operators (elf_amd/policy_ops.py): element types, activations, outputs
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ACTS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
-OUT_KINDS = {"logits": 0, "log_probs": 1, "probs": 2}
-
-
+# Argument blocks of the policy-network operators (torch callers: elf_amd/policy_ops.py)
 class Norm(C.Structure):
     """goenv_norm: the arguments that goenv_group_norm_act and its gradient share."""
     _fields_ = ([(k, C.c_int32) for k in ("device", "dtype", "param_dtype", "act")] +
