@@ -636,21 +636,45 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint32_t step, uint32_t 
 }
 
 template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+
+// A block of eight elements a thread and turn; VECTOR: the arrays allow 16-byte accesses.
+template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_dropout(int64_t n, const T* x, const T* residual, T* y, uint32_t thr, float scale,
                                                  const int64_t* rng, uint32_t site) {
   const uint64_t seed = (uint64_t)rng[0];
   const uint32_t step = (uint32_t)rng[1];
   for (int64_t blk = (int64_t)blockIdx.x * 256 + threadIdx.x; blk < (n + 7) / 8; blk += (int64_t)gridDim.x * 256) {
-    const uint4 u = philox((uint64_t)blk, step, site, seed);
+    const int64_t e = blk * 8;
+    const bool whole = VECTOR && e + 8 <= n;
+    Eight<T> a, r;
+    if (whole) {
+      a = *reinterpret_cast<const Eight<T>*>(x + e);
+      if (residual) r = *reinterpret_cast<const Eight<T>*>(residual + e);
+    }
+    const uint4 u = philox((uint64_t)blk, step, site, seed);   // under way while the loads are
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    auto keep = [&](int j) { return (j < 4 ? w[j] & 0xffffu : w[j - 4] >> 16) >= thr; };
+    if (whole) {
+      Eight<T> o;
+      if (residual) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t e = blk * 8 + j;
-      if (e >= n) break;
-      const uint32_t bits = j < 4 ? w[j] & 0xffffu : w[j - 4] >> 16;
-      float v = bits >= thr ? (float)x[e] * scale : 0.f;
-      if (residual) v += (float)residual[e];
-      y[e] = (T)v;
+        for (int j = 0; j < 8; ++j) o.v[j] = (T)((keep(j) ? (float)a.v[j] * scale : 0.f) + (float)r.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.v[j] = (T)(keep(j) ? (float)a.v[j] * scale : 0.f);
+      }
+      *reinterpret_cast<Eight<T>*>(y + e) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (e + j >= n) break;
+        float v = keep(j) ? (float)x[e + j] * scale : 0.f;
+        if (residual) v += (float)residual[e + j];
+        y[e + j] = (T)v;
+      }
     }
   }
 }
@@ -664,8 +688,24 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t n, const T* x, const T*
 // reading the logits a second time (from the caches) instead of writing and reading z in 32 bits.
 
 struct LogitCut {
+  int threads;             // of a slice
   int slices, per_group;   // slices of a row; rows that one workgroup takes one after the other
   int64_t groups;          // of rows
+};
+// The threads that share a slice: a workgroup, or (WAVE) one of its waves -- short rows go four to a workgroup, without barriers.
+template <bool WAVE>
+struct Team {
+  int tid, threads;
+  __device__ explicit Team(const LogitCut& cut) : tid(WAVE ? threadIdx.x & 63 : threadIdx.x), threads(cut.threads) {}
+  __device__ __forceinline__ int64_t index() const { return WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x; }
+  __device__ __forceinline__ void sync() const {
+    if (WAVE) {   // a wave's accesses to LDS keep their order; the compiler has to keep it too
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  }
 };
 enum LogitMode { LOGIT_MAP, LOGIT_WHOLE, LOGIT_SUMS, LOGIT_APPLY };   // no softmax; softmax in one launch, or in two
 
@@ -726,8 +766,8 @@ __device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, con
 
 // This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end), and dz / dlogit without the
 // temperature.  count: LDS, a word per column of the slice; every thread of the workgroup calls.
-template <typename T, int VEC, int NI>
-__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const RowRules& r, int64_t row, int v0, const int (&col)[NI],
+template <typename T, int VEC, int NI, bool WAVE>
+__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, const RowRules& r, int64_t row, int v0, const int (&col)[NI],
                                          const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
   load_columns<T, VEC, NI>(P.logits, sizeof(T) == 4, row * P.logits_row, col, z);
   uint32_t mask[NI];
@@ -745,32 +785,34 @@ __device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const RowRu
   float bias[NI][VEC];
   if (P.bias) load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, row * P.bias_row, col, bias);
   if (P.history) {
-    __syncthreads();   // the row before has read its counts
+    int len = P.history_len ? P.history_len[row] : P.history_max;
+    len = len < 0 ? 0 : len > P.history_max ? P.history_max : len;
+    team.sync();   // the row before has read its counts
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) count[(k * blockDim.x + threadIdx.x) * VEC + j] = 0;
-    __syncthreads();
-    int len = P.history_len ? P.history_len[row] : P.history_max;
-    len = len < 0 ? 0 : len > P.history_max ? P.history_max : len;
-    const int width = NI * VEC * blockDim.x;
-    auto mark = [&](int64_t v) {
-      const int64_t at = v - v0;
-      if (at >= 0 && at < width && v < P.cols) atomicAdd(&count[at], 1);
+      for (int j = 0; j < VEC; ++j) count[(k * team.threads + team.tid) * VEC + j] = 0;
+    team.sync();
+    // four entries at a time: their loads are under way together
+    auto scan = [&](auto* h) {
+      const int64_t end = v0 + (int64_t)NI * VEC * team.threads < P.cols ? v0 + (int64_t)NI * VEC * team.threads : P.cols;
+      for (int k = team.tid; k < len; k += 4 * team.threads) {
+        int64_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = h[(int64_t)k + i * team.threads < len ? k + i * team.threads : len - 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((int64_t)k + i * team.threads < len && v[i] >= v0 && v[i] < end) atomicAdd(&count[v[i] - v0], 1);
+      }
     };
-    if (P.history_i64) {
-      const int64_t* h = static_cast<const int64_t*>(P.history) + row * P.history_row;
-      for (int k = threadIdx.x; k < len; k += blockDim.x) mark(h[k]);
-    } else {
-      const int32_t* h = static_cast<const int32_t*>(P.history) + row * P.history_row;
-      for (int k = threadIdx.x; k < len; k += blockDim.x) mark(h[k]);
-    }
-    __syncthreads();
+    if (P.history_i64) scan(static_cast<const int64_t*>(P.history) + row * P.history_row);
+    else scan(static_cast<const int32_t*>(P.history) + row * P.history_row);
+    team.sync();
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const int c = count[(k * blockDim.x + threadIdx.x) * VEC + j];
+        const int c = count[(k * team.threads + team.tid) * VEC + j];
         const float l = z[k][j], f = l > 0.f ? r.inv_rep : r.rep;
         slope[k][j] = c > 0 ? f : 1.f;
         z[k][j] = c > 0 ? l * f - r.presence - r.frequency * (float)c : l;
@@ -796,13 +838,13 @@ __device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const RowRu
     }
 }
 
-// Over a workgroup of any number of waves, the same order every time.  lds: 16 floats.
-template <typename F>
-__device__ __forceinline__ float block_join(float v, float* lds, F f) {
+// Over a team, the same order every time.  lds: 16 floats.
+template <bool WAVE, typename F>
+__device__ __forceinline__ float team_join(const Team<WAVE>&, float v, float* lds, F f) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v = f(v, __shfl_xor(v, d));
+  if (WAVE) return v;
   const int waves = blockDim.x >> 6;
-  if (waves == 1) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -812,28 +854,31 @@ __device__ __forceinline__ float block_join(float v, float* lds, F f) {
 }
 __device__ __forceinline__ float add_f(float a, float b) { return a + b; }
 
-template <int VEC, int NI>
-__device__ __forceinline__ void columns_of(const goenv_logit_rules& P, int v0, int (&col)[NI], bool (&in)[NI]) {
+template <int VEC, int NI, bool WAVE>
+__device__ __forceinline__ void columns_of(const goenv_logit_rules& P, const Team<WAVE>& team, int v0, int (&col)[NI], bool (&in)[NI]) {
 #pragma unroll
   for (int k = 0; k < NI; ++k) {
-    const int64_t v = v0 + (int64_t)(k * blockDim.x + threadIdx.x) * VEC;
+    const int64_t v = v0 + (int64_t)(k * team.threads + team.tid) * VEC;
     in[k] = v < P.cols;
     col[k] = in[k] ? (int)v : (int)P.cols - VEC;
   }
 }
 
 // The workspace of the two launches: a row's slices' (largest z, sum exp(z - largest)).
-template <typename T, int VEC, int NI, int MODE>
+template <typename T, int VEC, int NI, bool WAVE, int MODE>
 __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, LogitCut cut, void* out) {
-  extern __shared__ __align__(16) int count[];
+  extern __shared__ __align__(16) int counts[];
   __shared__ float lds[16];
-  const int64_t row = blockIdx.x / (uint32_t)cut.slices;
-  const int slice = (int)(blockIdx.x % (uint32_t)cut.slices), v0 = slice * NI * VEC * (int)blockDim.x;
+  const Team<WAVE> team(cut);
+  const int64_t row = team.index() / cut.slices;
+  if (WAVE && row >= P.rows) return;
+  const int slice = (int)(team.index() % cut.slices), v0 = slice * NI * VEC * team.threads;
+  int* count = counts + (WAVE ? (threadIdx.x >> 6) * NI * VEC * 64 : 0);
   int col[NI];
   bool in[NI];
-  columns_of<VEC, NI>(P, v0, col, in);
+  columns_of<VEC, NI>(P, team, v0, col, in);
   float z[NI][VEC], slope[NI][VEC];
-  slice_of<T, VEC, NI>(P, rules_of(P, row), row, v0, col, in, count, z, slope);
+  slice_of<T, VEC, NI>(P, team, rules_of(P, row), row, v0, col, in, count, z, slope);
   if (MODE != LOGIT_MAP) {
     float m = -INFINITY, s = 0.f;
     if (MODE != LOGIT_APPLY) {
@@ -841,17 +886,17 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) m = fmaxf(m, z[k][j]);
-      m = block_join(m, lds, fmaxf);
+      m = team_join(team, m, lds, fmaxf);
       if (m == -INFINITY) m = 0.f;    // nothing left: every exponential is 0
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += __expf(z[k][j] - m);
-      s = block_join(s, lds, add_f);
+      s = team_join(team, s, lds, add_f);
     }
     float2* part = static_cast<float2*>(P.workspace) + row * cut.slices;
     if (MODE == LOGIT_SUMS) {
-      if (threadIdx.x == 0) part[slice] = make_float2(s == 0.f ? -INFINITY : m, s);
+      if (team.tid == 0) part[slice] = make_float2(s == 0.f ? -INFINITY : m, s);
       return;
     }
     if (MODE == LOGIT_APPLY) {
@@ -865,7 +910,7 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
     }
-    if (P.stats && slice == 0 && threadIdx.x == 0) {
+    if (P.stats && slice == 0 && team.tid == 0) {
       P.stats[2 * row] = m;
       P.stats[2 * row + 1] = s;
     }
@@ -884,16 +929,19 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
 
 // The gradients.  The workspace: a row's slices' sums of dy (log probabilities) or p dy (probabilities), then the row groups'
 // sums of dz for a bias that all rows share.
-template <typename T, int VEC, int NI, int MODE>
+template <typename T, int VEC, int NI, bool WAVE, int MODE>
 __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P, LogitCut cut, const void* d_out, int64_t dy_row, T* dlogits,
                                                              void* dbias, float* shared) {
-  extern __shared__ __align__(16) int count[];
+  extern __shared__ __align__(16) int counts[];
   __shared__ float lds[16];
-  const int64_t group = blockIdx.x / (uint32_t)cut.slices;
-  const int slice = (int)(blockIdx.x % (uint32_t)cut.slices), v0 = slice * NI * VEC * (int)blockDim.x;
+  const Team<WAVE> team(cut);
+  const int64_t group = team.index() / cut.slices;
+  if (WAVE && group >= cut.groups) return;
+  const int slice = (int)(team.index() % cut.slices), v0 = slice * NI * VEC * team.threads;
+  int* count = counts + (WAVE ? (threadIdx.x >> 6) * NI * VEC * 64 : 0);
   int col[NI];
   bool in[NI];
-  columns_of<VEC, NI>(P, v0, col, in);
+  columns_of<VEC, NI>(P, team, v0, col, in);
   float sum[NI][VEC];
 #pragma unroll
   for (int k = 0; k < NI; ++k)
@@ -904,7 +952,7 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
     const RowRules r = rules_of(P, row);
     float z[NI][VEC], slope[NI][VEC], dz[NI][VEC];
     load_columns<T, VEC, NI>(d_out, P.out_dtype == GOENV_DT_F32, row * dy_row, col, dz);
-    slice_of<T, VEC, NI>(P, r, row, v0, col, in, count, z, slope);
+    slice_of<T, VEC, NI>(P, team, r, row, v0, col, in, count, z, slope);
     if (MODE != LOGIT_MAP) {
       const float m = P.stats[2 * row], inv_s = 1.f / P.stats[2 * row + 1];
       const bool probs = P.out_kind == GOENV_OUT_PROBS;
@@ -927,10 +975,10 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
       } else {
-        total = block_join(total, lds, add_f);
+        total = team_join(team, total, lds, add_f);
       }
       if (MODE == LOGIT_SUMS) {
-        if (threadIdx.x == 0) part[slice] = total;
+        if (team.tid == 0) part[slice] = total;
         continue;
       }
 #pragma unroll
@@ -1094,7 +1142,8 @@ void by_vec(int vec, F f) {
 struct LogitPlan {
   LogitCut cut;
   int threads, vec, ni;
-  bool split;
+  bool split, wave;   // wave: a wave a slice, four a workgroup
+  unsigned blocks(int64_t teams) const { return (unsigned)(wave ? (teams + 3) / 4 : teams); }
 };
 
 // The cut for vectors of `vec` columns (which goes by the arrays' alignment: a workspace is sized for either).  The gradient holds four
@@ -1107,7 +1156,10 @@ LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, bool
   p.split = softmax && cols > 1024 * each;
   p.threads = 64;
   while (p.threads < (p.split || !softmax ? 256 : 1024) && (int64_t)p.threads * each < cols) p.threads *= 2;
-  p.cut.slices = (int)((cols + (int64_t)p.threads * each - 1) / ((int64_t)p.threads * each));
+  p.cut.threads = p.threads;
+  p.wave = p.threads == 64;
+  if (p.wave) p.threads = 256;
+  p.cut.slices = (int)((cols + (int64_t)p.cut.threads * each - 1) / ((int64_t)p.cut.threads * each));
   p.cut.per_group = 1;
   if (shared) {
     const int64_t wgs = rows * p.cut.slices, most = rows < 65536 ? rows : 65536;
@@ -1300,8 +1352,12 @@ int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* r
   const float scale = thr >= 65536u ? 0.f : (float)(65536. / (65536. - thr));
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_dropout<T>), dim3(grid_of(((n + 7) / 8 + 255) / 256)), dim3(256), 0, S(stream), n, static_cast<const T*>(x),
-                       static_cast<const T*>(residual), static_cast<T*>(y), thr, scale, rng, site);
+    const bool vector = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) & 15) == 0;
+    auto go = [&](auto f) {
+      hipLaunchKernelGGL(f, dim3(grid_of(((n + 7) / 8 + 255) / 256)), dim3(256), 0, S(stream), n, static_cast<const T*>(x),
+                         static_cast<const T*>(residual), static_cast<T*>(y), thr, scale, rng, site);
+    };
+    vector ? go(k_dropout<T, true>) : go(k_dropout<T, false>);
   });
   HIPCHK(hipGetLastError());
   return 0;
@@ -1334,15 +1390,15 @@ int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream) {
       constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
       const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
       auto go = [&](auto f) {
-        hipLaunchKernelGGL(f, dim3((unsigned)(p->rows * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, out);
+        hipLaunchKernelGGL(f, dim3(plan.blocks(p->rows * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, out);
       };
       if (!softmax) {
-        go(k_policy_logits<T, VEC, NI, LOGIT_MAP>);
+        plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_MAP>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_MAP>);
       } else if (!plan.split) {
-        go(k_policy_logits<T, VEC, NI, LOGIT_WHOLE>);
+        plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_WHOLE>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_WHOLE>);
       } else {
-        go(k_policy_logits<T, VEC, NI, LOGIT_SUMS>);
-        go(k_policy_logits<T, VEC, NI, LOGIT_APPLY>);
+        go(k_policy_logits<T, VEC, NI, false, LOGIT_SUMS>);
+        go(k_policy_logits<T, VEC, NI, false, LOGIT_APPLY>);
       }
     };
     plan.vec == 4 ? with(Int<4>(), Int<4>()) : with(Int<1>(), Int<6>());
@@ -1371,16 +1427,16 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
         constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
         const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
         auto go = [&](auto f) {
-          hipLaunchKernelGGL(f, dim3((unsigned)(plan.cut.groups * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, d_out,
+          hipLaunchKernelGGL(f, dim3(plan.blocks(plan.cut.groups * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, d_out,
                              dy_row, static_cast<T*>(dlogits), dbias, parts);
         };
         if (!softmax) {
-          go(k_policy_logits_grad<T, VEC, NI, LOGIT_MAP>);
+          plan.wave ? go(k_policy_logits_grad<T, VEC, NI, true, LOGIT_MAP>) : go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_MAP>);
         } else if (!plan.split) {
-          go(k_policy_logits_grad<T, VEC, NI, LOGIT_WHOLE>);
+          plan.wave ? go(k_policy_logits_grad<T, VEC, NI, true, LOGIT_WHOLE>) : go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_WHOLE>);
         } else {
-          go(k_policy_logits_grad<T, VEC, NI, LOGIT_SUMS>);
-          go(k_policy_logits_grad<T, VEC, NI, LOGIT_APPLY>);
+          go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_SUMS>);
+          go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_APPLY>);
         }
       };
       plan.vec == 4 ? with(Int<4>(), Int<2>()) : with(Int<1>(), Int<6>());
