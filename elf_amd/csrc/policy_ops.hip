@@ -32,29 +32,37 @@ __device__ __forceinline__ void store_any(void* p, int dt, int64_t i, float v) {
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
+// A wave's lanes joined by f, in the same order every time, for every lane: scans along rows of 16 lanes, then across the rows (the
+// last lane has seen all).  Register moves between lanes; an exchange through LDS takes ten times as long.
+template <int CTRL, int ROWS, typename F>
+__device__ __forceinline__ float join_step(float v, float none, F f) {
+  return f(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false)));
+}
+template <typename F>
+__device__ __forceinline__ float wave_join(float v, float none, F f) {
+  v = join_step<0x111, 0xf>(v, none, f);   // from 1, 2, 4 and 8 lanes before in the row
+  v = join_step<0x112, 0xf>(v, none, f);
+  v = join_step<0x114, 0xf>(v, none, f);
+  v = join_step<0x118, 0xf>(v, none, f);
+  v = join_step<0x142, 0xa>(v, none, f);   // the last lane of rows 0 and 2 to rows 1 and 3
+  v = join_step<0x143, 0xc>(v, none, f);   // lane 31 to rows 2 and 3
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_join(v, 0.f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v) { return wave_join(v, -INFINITY, fmaxf); }
+
 // Sum over a workgroup of WAVES waves, in the same order every time; every thread gets it.
 template <int WAVES>
 __device__ __forceinline__ float block_sum(float v, float* lds) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   float t = 0.f;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) t += lds[w];
-  return t;
-}
-template <int WAVES>
-__device__ __forceinline__ float block_max(float v, float* lds) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = lds[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) t = fmaxf(t, lds[w]);
   return t;
 }
 
@@ -205,8 +213,7 @@ __device__ __forceinline__ void slab_sum(const NormCut& cut, int cpg, const Norm
       const int row = k / mine;
       v += lds[row * cut.units * NV + g * mine + (k - row * mine)];
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    v = wave_sum(v);
     if (lane == 0) total[g] = v;
   }
   __syncthreads();
@@ -309,15 +316,13 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm(goenv_norm P, NormC
       auto size = [&](int k) { return (float)((k + 1) * cut.chunk < P.positions ? cut.chunk : P.positions - k * cut.chunk) * (float)cpg; };
       float m = 0.f, s = 0.f;
       for (int k = lane; k < cut.chunks; k += 64) m += size(k) * part[k].x;
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) m += __shfl_xor(m, d);
+      m = wave_sum(m);
       m *= inv_m;
       for (int k = lane; k < cut.chunks; k += 64) {
         const float2 v = part[k];
         s += v.y + size(k) * (v.x - m) * (v.x - m);
       }
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+      s = wave_sum(s);
       s = 1.f / sqrtf(s * inv_m + P.eps);
       if (lane == 0) {
         lds[2 * g] = m;
@@ -472,11 +477,8 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
       m1 += sum1[g * cpg + k];
       m2 += sum2[g * cpg + k];
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      m1 += __shfl_xor(m1, d);
-      m2 += __shfl_xor(m2, d);
-    }
+    m1 = wave_sum(m1);
+    m2 = wave_sum(m2);
     const float inv_m = 1.f / ((float)P.positions * (float)cpg);
     if (lane == 0) {
       group[2 * g] = m1 * inv_m;
@@ -696,8 +698,12 @@ struct LogitCut {
 template <bool WAVE>
 struct Team {
   int tid, threads;
-  __device__ explicit Team(const LogitCut& cut) : tid(WAVE ? threadIdx.x & 63 : threadIdx.x), threads(cut.threads) {}
-  __device__ __forceinline__ int64_t index() const { return WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x; }
+  uint32_t index;
+  __device__ __forceinline__ explicit Team(const LogitCut& cut) : tid(WAVE ? threadIdx.x & 63 : threadIdx.x), threads(WAVE ? 64 : cut.threads) {
+    index = WAVE ? blockIdx.x * 4 + wave() : blockIdx.x;
+  }
+  // (the same for all lanes, and known to be: a row's addresses and rules are scalars)
+  __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
   __device__ __forceinline__ void sync() const {
     if (WAVE) {   // a wave's accesses to LDS keep their order; the compiler has to keep it too
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -705,6 +711,25 @@ struct Team {
     } else {
       __syncthreads();
     }
+  }
+  // Over the team, the same order every time.  lds: 16 floats.
+  __device__ __forceinline__ float sum(float v, float* lds) const {
+    v = wave_sum(v);
+    return WAVE ? v : across(v, lds, [](float a, float b) { return a + b; });
+  }
+  __device__ __forceinline__ float max(float v, float* lds) const {
+    v = wave_max(v);
+    return WAVE ? v : across(v, lds, fmaxf);
+  }
+  template <typename F>
+  __device__ __forceinline__ float across(float v, float* lds, F f) const {
+    const int waves = threads >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+    for (int w = 1; w < waves; ++w) v = f(v, lds[w]);
+    return v;
   }
 };
 enum LogitMode { LOGIT_MAP, LOGIT_WHOLE, LOGIT_SUMS, LOGIT_APPLY };   // no softmax; softmax in one launch, or in two
@@ -724,11 +749,11 @@ __device__ __forceinline__ RowRules rules_of(const goenv_logit_rules& P, int64_t
 
 // NI vectors of an array of type F32 or T.  The columns behind the last vector read that one again.
 template <typename T, int VEC, int NI>
-__device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at, const int (&col)[NI], float (&to)[NI][VEC]) {
+__device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at, const uint32_t (&col)[NI], float (&to)[NI][VEC]) {
   if (f32) {
     Pack<float, VEC> v[NI];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) v[k] = load_pack<float, VEC>(static_cast<const float*>(p) + at + col[k]);
+    for (int k = 0; k < NI; ++k) v[k] = load_pack<float, VEC>(static_cast<const float*>(p) + at + (size_t)col[k]);
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
@@ -736,7 +761,7 @@ __device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at
   } else {
     Pack<T, VEC> v[NI];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) v[k] = load_pack<T, VEC>(static_cast<const T*>(p) + at + col[k]);
+    for (int k = 0; k < NI; ++k) v[k] = load_pack<T, VEC>(static_cast<const T*>(p) + at + (size_t)col[k]);
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
@@ -744,7 +769,7 @@ __device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at
   }
 }
 template <typename T, int VEC, int NI>
-__device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, const int (&col)[NI], const bool (&in)[NI], const float (&from)[NI][VEC]) {
+__device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, const uint32_t (&col)[NI], const bool (&in)[NI], const float (&from)[NI][VEC]) {
   if (f32) {
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
@@ -767,7 +792,7 @@ __device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, con
 // This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end), and dz / dlogit without the
 // temperature.  count: LDS, a word per column of the slice; every thread of the workgroup calls.
 template <typename T, int VEC, int NI, bool WAVE>
-__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, const RowRules& r, int64_t row, int v0, const int (&col)[NI],
+__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, const RowRules& r, int64_t row, int v0, const uint32_t (&col)[NI],
                                          const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
   load_columns<T, VEC, NI>(P.logits, sizeof(T) == 4, row * P.logits_row, col, z);
   uint32_t mask[NI];
@@ -795,14 +820,14 @@ __device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<
     team.sync();
     // four entries at a time: their loads are under way together
     auto scan = [&](auto* h) {
-      const int64_t end = v0 + (int64_t)NI * VEC * team.threads < P.cols ? v0 + (int64_t)NI * VEC * team.threads : P.cols;
+      const uint32_t width = (uint32_t)(NI * VEC * team.threads), left = (uint32_t)P.cols - v0, most = width < left ? width : left;
       for (int k = team.tid; k < len; k += 4 * team.threads) {
         int64_t v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = h[(int64_t)k + i * team.threads < len ? k + i * team.threads : len - 1];
+        for (int i = 0; i < 4; ++i) v[i] = h[k + i * team.threads < len ? k + i * team.threads : len - 1];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if ((int64_t)k + i * team.threads < len && v[i] >= v0 && v[i] < end) atomicAdd(&count[v[i] - v0], 1);
+          if (k + i * team.threads < len && v[i] >= v0 && v[i] - v0 < most) atomicAdd(&count[v[i] - v0], 1);
       }
     };
     if (P.history_i64) scan(static_cast<const int64_t*>(P.history) + row * P.history_row);
@@ -838,29 +863,13 @@ __device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<
     }
 }
 
-// Over a team, the same order every time.  lds: 16 floats.
-template <bool WAVE, typename F>
-__device__ __forceinline__ float team_join(const Team<WAVE>&, float v, float* lds, F f) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = f(v, __shfl_xor(v, d));
-  if (WAVE) return v;
-  const int waves = blockDim.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0];
-  for (int w = 1; w < waves; ++w) v = f(v, lds[w]);
-  return v;
-}
-__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
-
 template <int VEC, int NI, bool WAVE>
-__device__ __forceinline__ void columns_of(const goenv_logit_rules& P, const Team<WAVE>& team, int v0, int (&col)[NI], bool (&in)[NI]) {
+__device__ __forceinline__ void columns_of(const goenv_logit_rules& P, const Team<WAVE>& team, int v0, uint32_t (&col)[NI], bool (&in)[NI]) {
 #pragma unroll
   for (int k = 0; k < NI; ++k) {
-    const int64_t v = v0 + (int64_t)(k * team.threads + team.tid) * VEC;
-    in[k] = v < P.cols;
-    col[k] = in[k] ? (int)v : (int)P.cols - VEC;
+    const uint32_t v = (uint32_t)v0 + (uint32_t)(k * team.threads + team.tid) * VEC, cols = (uint32_t)P.cols;
+    in[k] = v < cols;
+    col[k] = in[k] ? v : cols - VEC;
   }
 }
 
@@ -870,11 +879,12 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
   extern __shared__ __align__(16) int counts[];
   __shared__ float lds[16];
   const Team<WAVE> team(cut);
-  const int64_t row = team.index() / cut.slices;
+  const uint32_t slices = cut.slices, at = team.index / slices;
+  const int64_t row = at;
   if (WAVE && row >= P.rows) return;
-  const int slice = (int)(team.index() % cut.slices), v0 = slice * NI * VEC * team.threads;
-  int* count = counts + (WAVE ? (threadIdx.x >> 6) * NI * VEC * 64 : 0);
-  int col[NI];
+  const int slice = (int)(team.index - at * slices), v0 = slice * NI * VEC * team.threads;
+  int* count = counts + (WAVE ? team.wave() * NI * VEC * 64 : 0);
+  uint32_t col[NI];
   bool in[NI];
   columns_of<VEC, NI>(P, team, v0, col, in);
   float z[NI][VEC], slope[NI][VEC];
@@ -886,13 +896,13 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) m = fmaxf(m, z[k][j]);
-      m = team_join(team, m, lds, fmaxf);
+      m = team.max(m, lds);
       if (m == -INFINITY) m = 0.f;    // nothing left: every exponential is 0
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += __expf(z[k][j] - m);
-      s = team_join(team, s, lds, add_f);
+      s = team.sum(s, lds);
     }
     float2* part = static_cast<float2*>(P.workspace) + row * cut.slices;
     if (MODE == LOGIT_SUMS) {
@@ -903,12 +913,10 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
       // every wave joins the slices by itself
       const int lane = threadIdx.x & 63;
       for (int k = lane; k < cut.slices; k += 64) m = fmaxf(m, part[k].x);
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+      m = wave_max(m);
       if (m == -INFINITY) m = 0.f;
       for (int k = lane; k < cut.slices; k += 64) s += part[k].y == 0.f ? 0.f : part[k].y * __expf(part[k].x - m);
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+      s = wave_sum(s);
     }
     if (P.stats && slice == 0 && team.tid == 0) {
       P.stats[2 * row] = m;
@@ -935,11 +943,12 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
   extern __shared__ __align__(16) int counts[];
   __shared__ float lds[16];
   const Team<WAVE> team(cut);
-  const int64_t group = team.index() / cut.slices;
+  const uint32_t slices = cut.slices, at = team.index / slices;
+  const int64_t group = at;
   if (WAVE && group >= cut.groups) return;
-  const int slice = (int)(team.index() % cut.slices), v0 = slice * NI * VEC * team.threads;
-  int* count = counts + (WAVE ? (threadIdx.x >> 6) * NI * VEC * 64 : 0);
-  int col[NI];
+  const int slice = (int)(team.index - at * slices), v0 = slice * NI * VEC * team.threads;
+  int* count = counts + (WAVE ? team.wave() * NI * VEC * 64 : 0);
+  uint32_t col[NI];
   bool in[NI];
   columns_of<VEC, NI>(P, team, v0, col, in);
   float sum[NI][VEC];
@@ -972,10 +981,9 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
       if (MODE == LOGIT_APPLY) {
         total = 0.f;
         for (int k = threadIdx.x & 63; k < cut.slices; k += 64) total += part[k];
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+        total = wave_sum(total);
       } else {
-        total = team_join(team, total, lds, add_f);
+        total = team.sum(total, lds);
       }
       if (MODE == LOGIT_SUMS) {
         if (team.tid == 0) part[slice] = total;
@@ -1216,9 +1224,9 @@ int check_logits(const goenv_logit_rules* p, bool grad) {
   if (p->bias && p->bias_dtype != GOENV_DT_F32 && p->bias_dtype != p->dtype)
     return fail("goenv_policy_logits: bias_dtype must be GOENV_DT_F32 or dtype");
   if (p->out_kind < GOENV_OUT_LOGITS || p->out_kind > GOENV_OUT_PROBS) return fail("goenv_policy_logits: out_kind must be a GOENV_OUT_*");
-  if (p->rows < 0 || p->cols < 0 || p->cols > INT32_MAX) return fail("goenv_policy_logits: rows or cols out of range");
+  if (p->rows < 0 || p->cols < 0 || p->cols > (1 << 30)) return fail("goenv_policy_logits: rows or cols out of range");
   if (p->legal && p->legal_bits) return fail("goenv_policy_logits: legal or legal_bits, not both");
-  if (p->history && p->history_max < 0) return fail("goenv_policy_logits: history_max is negative");
+  if (p->history && (p->history_max < 0 || p->history_max > (1 << 30))) return fail("goenv_policy_logits: history_max out of range");
   if (!p->row_temperature && !(p->temperature > 0.f && isfinite(p->temperature)))
     return fail("goenv_policy_logits: temperature must be positive and finite");
   if (p->history) {
