@@ -5,6 +5,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/goenv.h"
 #include "goenv_host.h"
 
@@ -739,95 +741,116 @@ struct RowRules {
 };
 __device__ __forceinline__ RowRules rules_of(const goenv_logit_rules& P, int64_t row) {
   RowRules r;
-  r.rep = P.row_repetition ? P.row_repetition[row] : P.repetition;
-  r.presence = P.row_presence ? P.row_presence[row] : P.presence;
-  r.frequency = P.row_frequency ? P.row_frequency[row] : P.frequency;
+  float t;
+  if (P.row_repetition && P.row_presence && P.row_frequency && P.row_temperature) {   // the loads are under way together
+    r.rep = P.row_repetition[row];
+    r.presence = P.row_presence[row];
+    r.frequency = P.row_frequency[row];
+    t = P.row_temperature[row];
+  } else {
+    r.rep = P.row_repetition ? P.row_repetition[row] : P.repetition;
+    r.presence = P.row_presence ? P.row_presence[row] : P.presence;
+    r.frequency = P.row_frequency ? P.row_frequency[row] : P.frequency;
+    t = P.row_temperature ? P.row_temperature[row] : P.temperature;
+  }
   r.inv_rep = 1.f / r.rep;
-  r.inv_t = 1.f / (P.row_temperature ? P.row_temperature[row] : P.temperature);
+  r.inv_t = 1.f / t;
   return r;
 }
 
-// NI vectors of an array of type F32 or T.  The columns behind the last vector read that one again.
+// A row's start (a scalar) and an offset in bytes below 2^32: one addition to a load
+template <typename P>
+__device__ __forceinline__ P* in_row(const void* row, uint32_t bytes) {
+  return reinterpret_cast<P*>(const_cast<char*>(static_cast<const char*>(row)) + bytes);
+}
+
+// NI vectors of an array of type F32 or T, the row at element `at`.  The columns behind the last vector read that one again.
+template <typename E, int VEC, int NI>
+__device__ __forceinline__ void load_row(const E* row, const uint32_t (&col)[NI], float (&to)[NI][VEC]) {
+  Pack<E, VEC> v[NI];
+#pragma unroll
+  for (int k = 0; k < NI; ++k) v[k] = *in_row<const Pack<E, VEC>>(row, col[k] * (uint32_t)sizeof(E));
+#pragma unroll
+  for (int k = 0; k < NI; ++k)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) to[k][j] = (float)v[k].v[j];
+}
 template <typename T, int VEC, int NI>
 __device__ __forceinline__ void load_columns(const void* p, bool f32, int64_t at, const uint32_t (&col)[NI], float (&to)[NI][VEC]) {
-  if (f32) {
-    Pack<float, VEC> v[NI];
+  if (f32) load_row<float, VEC, NI>(static_cast<const float*>(p) + at, col, to);
+  else load_row<T, VEC, NI>(static_cast<const T*>(p) + at, col, to);
+}
+template <typename E, int VEC, int NI>
+__device__ __forceinline__ void store_row(E* row, const uint32_t (&col)[NI], const bool (&in)[NI], const float (&from)[NI][VEC]) {
 #pragma unroll
-    for (int k = 0; k < NI; ++k) v[k] = load_pack<float, VEC>(static_cast<const float*>(p) + at + (size_t)col[k]);
+  for (int k = 0; k < NI; ++k) {
+    Pack<E, VEC> v;
 #pragma unroll
-    for (int k = 0; k < NI; ++k)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) to[k][j] = v[k].v[j];
-  } else {
-    Pack<T, VEC> v[NI];
-#pragma unroll
-    for (int k = 0; k < NI; ++k) v[k] = load_pack<T, VEC>(static_cast<const T*>(p) + at + (size_t)col[k]);
-#pragma unroll
-    for (int k = 0; k < NI; ++k)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) to[k][j] = (float)v[k].v[j];
+    for (int j = 0; j < VEC; ++j) v.v[j] = (E)from[k][j];
+    if (in[k]) *in_row<Pack<E, VEC>>(row, col[k] * (uint32_t)sizeof(E)) = v;
   }
 }
 template <typename T, int VEC, int NI>
 __device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, const uint32_t (&col)[NI], const bool (&in)[NI], const float (&from)[NI][VEC]) {
-  if (f32) {
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      Pack<float, VEC> v;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v.v[j] = from[k][j];
-      if (in[k]) *reinterpret_cast<Pack<float, VEC>*>(static_cast<float*>(p) + at + col[k]) = v;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      Pack<T, VEC> v;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v.v[j] = (T)from[k][j];
-      if (in[k]) *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(p) + at + col[k]) = v;
-    }
-  }
+  if (f32) store_row<float, VEC, NI>(static_cast<float*>(p) + at, col, in, from);
+  else store_row<T, VEC, NI>(static_cast<T*>(p) + at, col, in, from);
 }
 
 // This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end), and dz / dlogit without the
-// temperature.  count: LDS, a word per column of the slice; every thread of the workgroup calls.
+// temperature; returns 1 / temperature.  count: LDS, a word per column of the slice; every thread of the team calls.
+// All loads start before anything waits for one: a short row's time is the time of its longest chain of loads.
 template <typename T, int VEC, int NI, bool WAVE>
-__device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, const RowRules& r, int64_t row, int v0, const uint32_t (&col)[NI],
-                                         const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
-  load_columns<T, VEC, NI>(P.logits, sizeof(T) == 4, row * P.logits_row, col, z);
+__device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, int64_t row, uint32_t v0, const uint32_t (&col)[NI],
+                                          const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
+  const T* logits = static_cast<const T*>(P.logits) + row * P.logits_row;
+  Pack<T, VEC> raw[NI];
+#pragma unroll
+  for (int k = 0; k < NI; ++k) raw[k] = *in_row<const Pack<T, VEC>>(logits, col[k] * (uint32_t)sizeof(T));
   uint32_t mask[NI];
   if (P.legal) {
+    const uint8_t* legal = P.legal + row * P.legal_row;
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      const uint8_t* at = P.legal + row * P.legal_row + col[k];
-      if constexpr (VEC == 4) mask[k] = *reinterpret_cast<const uint32_t*>(at);
-      else mask[k] = *at;
-    }
+    for (int k = 0; k < NI; ++k) mask[k] = VEC == 4 ? *in_row<const uint32_t>(legal, col[k]) : *in_row<const uint8_t>(legal, col[k]);
   } else if (P.legal_bits) {
+    const uint32_t* bits = P.legal_bits + row * P.bits_row;
 #pragma unroll
-    for (int k = 0; k < NI; ++k) mask[k] = P.legal_bits[row * P.bits_row + (col[k] >> 5)];
+    for (int k = 0; k < NI; ++k) mask[k] = *in_row<const uint32_t>(bits, (col[k] >> 5) * 4);
   }
   float bias[NI][VEC];
   if (P.bias) load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, row * P.bias_row, col, bias);
-  if (P.history) {
-    int len = P.history_len ? P.history_len[row] : P.history_max;
-    len = len < 0 ? 0 : len > P.history_max ? P.history_max : len;
-    team.sync();   // the row before has read its counts
-#pragma unroll
-    for (int k = 0; k < NI; ++k)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) count[(k * team.threads + team.tid) * VEC + j] = 0;
-    team.sync();
-    // four entries at a time: their loads are under way together
+  const bool past = P.history && P.history_max > 0;
+  const uint32_t width = (uint32_t)(NI * VEC * team.threads), left = (uint32_t)P.cols - v0, most = width < left ? width : left;
+  RowRules r;
+  if (past) {
     auto scan = [&](auto* h) {
-      const uint32_t width = (uint32_t)(NI * VEC * team.threads), left = (uint32_t)P.cols - v0, most = width < left ? width : left;
-      for (int k = team.tid; k < len; k += 4 * team.threads) {
-        int64_t v[4];
+      using I = std::remove_const_t<std::remove_pointer_t<decltype(h)>>;
+      using U = std::make_unsigned_t<I>;
+      I v[4];
+      auto load = [&](int k) {   // four entries at a time
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = h[k + i * team.threads < len ? k + i * team.threads : len - 1];
+        for (int i = 0; i < 4; ++i) {
+          const int at = k + i * team.threads;
+          v[i] = *in_row<const I>(h, (uint32_t)(at < P.history_max ? at : P.history_max - 1) * (uint32_t)sizeof(I));
+        }
+      };
+      load(team.tid);            // before the row's length is here
+      int len = P.history_len ? P.history_len[row] : P.history_max;
+      len = len < 0 ? 0 : len > P.history_max ? P.history_max : len;
+      r = rules_of(P, row);
+      team.sync();               // the row before has read its counts
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (k + i * team.threads < len && v[i] >= v0 && v[i] - v0 < most) atomicAdd(&count[v[i] - v0], 1);
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) count[(k * team.threads + team.tid) * VEC + j] = 0;
+      team.sync();
+      for (int k = team.tid; k < len;) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const U at = (U)v[i] - (U)v0;   // (negative entries are far beyond every column)
+          if (k + i * team.threads < len && at < most) atomicAdd(&count[at], 1);
+        }
+        k += 4 * team.threads;
+        if (k < len) load(k);
       }
     };
     if (P.history_i64) scan(static_cast<const int64_t*>(P.history) + row * P.history_row);
@@ -838,29 +861,35 @@ __device__ __forceinline__ void slice_of(const goenv_logit_rules& P, const Team<
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const int c = count[(k * team.threads + team.tid) * VEC + j];
-        const float l = z[k][j], f = l > 0.f ? r.inv_rep : r.rep;
+        const float l = (float)raw[k].v[j], f = l > 0.f ? r.inv_rep : r.rep;
         slope[k][j] = c > 0 ? f : 1.f;
         z[k][j] = c > 0 ? l * f - r.presence - r.frequency * (float)c : l;
       }
   } else {
+    r = rules_of(P, row);
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) slope[k][j] = 1.f;
+      for (int j = 0; j < VEC; ++j) {
+        slope[k][j] = 1.f;
+        z[k][j] = (float)raw[k].v[j];
+      }
   }
   if (P.bias)
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) z[k][j] += bias[k][j];
-  const bool bytes = P.legal != nullptr, masked = bytes || P.legal_bits != nullptr;
+  auto finish = [&](auto allowed) {
 #pragma unroll
-  for (int k = 0; k < NI; ++k)
+    for (int k = 0; k < NI; ++k)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const uint32_t m = bytes ? mask[k] & (0xffu << (8 * j)) : mask[k] & (1u << ((col[k] + j) & 31));
-      z[k][j] = (masked && m == 0) || !in[k] ? -INFINITY : z[k][j] * r.inv_t;
-    }
+      for (int j = 0; j < VEC; ++j) z[k][j] = (int)allowed(k, j) & (int)in[k] ? z[k][j] * r.inv_t : -INFINITY;
+  };
+  if (P.legal) finish([&](int k, int j) { return (mask[k] & (0xffu << (8 * j))) != 0; });
+  else if (P.legal_bits) finish([&](int k, int j) { return ((mask[k] >> ((col[k] + j) & 31)) & 1u) != 0; });
+  else finish([](int, int) { return true; });
+  return r.inv_t;
 }
 
 template <int VEC, int NI, bool WAVE>
@@ -888,7 +917,7 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
   bool in[NI];
   columns_of<VEC, NI>(P, team, v0, col, in);
   float z[NI][VEC], slope[NI][VEC];
-  slice_of<T, VEC, NI>(P, team, rules_of(P, row), row, v0, col, in, count, z, slope);
+  slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, slope);
   if (MODE != LOGIT_MAP) {
     float m = -INFINITY, s = 0.f;
     if (MODE != LOGIT_APPLY) {
@@ -922,15 +951,19 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
       P.stats[2 * row] = m;
       P.stats[2 * row + 1] = s;
     }
-    const float log_s = logf(s), inv_s = 1.f / s;
-    const bool probs = P.out_kind == GOENV_OUT_PROBS;
+    if (P.out_kind == GOENV_OUT_PROBS) {
+      const float inv_s = 1.f / s;
 #pragma unroll
-    for (int k = 0; k < NI; ++k)
+      for (int k = 0; k < NI; ++k)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = z[k][j] - m;
-        z[k][j] = z[k][j] == -INFINITY ? (probs ? 0.f : -INFINITY) : probs ? __expf(d) * inv_s : d - log_s;
-      }
+        for (int j = 0; j < VEC; ++j) z[k][j] = z[k][j] == -INFINITY ? 0.f : __expf(z[k][j] - m) * inv_s;
+    } else {
+      const float log_s = logf(s);
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[k][j] = z[k][j] == -INFINITY ? -INFINITY : z[k][j] - m - log_s;
+    }
   }
   store_columns<T, VEC, NI>(out, P.out_dtype == GOENV_DT_F32, row * P.cols, col, in, z);
 }
@@ -958,10 +991,9 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
     for (int j = 0; j < VEC; ++j) sum[k][j] = 0.f;
   const int64_t end = (group + 1) * cut.per_group < P.rows ? (group + 1) * cut.per_group : P.rows;
   for (int64_t row = group * cut.per_group; row < end; ++row) {
-    const RowRules r = rules_of(P, row);
     float z[NI][VEC], slope[NI][VEC], dz[NI][VEC];
     load_columns<T, VEC, NI>(d_out, P.out_dtype == GOENV_DT_F32, row * dy_row, col, dz);
-    slice_of<T, VEC, NI>(P, team, r, row, v0, col, in, count, z, slope);
+    const float inv_t = slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, slope);
     if (MODE != LOGIT_MAP) {
       const float m = P.stats[2 * row], inv_s = 1.f / P.stats[2 * row + 1];
       const bool probs = P.out_kind == GOENV_OUT_PROBS;
@@ -999,7 +1031,7 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         if (MODE == LOGIT_MAP && z[k][j] == -INFINITY) dz[k][j] = slope[k][j] = 0.f;
-        dz[k][j] *= r.inv_t;
+        dz[k][j] *= inv_t;
         sum[k][j] += dz[k][j];
       }
     if (dbias && !shared) store_columns<T, VEC, NI>(dbias, P.bias_dtype == GOENV_DT_F32, row * P.cols, col, in, dz);
@@ -1224,9 +1256,9 @@ int check_logits(const goenv_logit_rules* p, bool grad) {
   if (p->bias && p->bias_dtype != GOENV_DT_F32 && p->bias_dtype != p->dtype)
     return fail("goenv_policy_logits: bias_dtype must be GOENV_DT_F32 or dtype");
   if (p->out_kind < GOENV_OUT_LOGITS || p->out_kind > GOENV_OUT_PROBS) return fail("goenv_policy_logits: out_kind must be a GOENV_OUT_*");
-  if (p->rows < 0 || p->cols < 0 || p->cols > (1 << 30)) return fail("goenv_policy_logits: rows or cols out of range");
+  if (p->rows < 0 || p->cols < 0 || p->cols > (1 << 28)) return fail("goenv_policy_logits: rows or cols out of range");
   if (p->legal && p->legal_bits) return fail("goenv_policy_logits: legal or legal_bits, not both");
-  if (p->history && (p->history_max < 0 || p->history_max > (1 << 30))) return fail("goenv_policy_logits: history_max out of range");
+  if (p->history && (p->history_max < 0 || p->history_max > (1 << 28))) return fail("goenv_policy_logits: history_max out of range");
   if (!p->row_temperature && !(p->temperature > 0.f && isfinite(p->temperature)))
     return fail("goenv_policy_logits: temperature must be positive and finite");
   if (p->history) {

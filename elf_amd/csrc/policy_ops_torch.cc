@@ -496,7 +496,7 @@ Tensor policy_logits(py::handle plogits, py::handle plegal, py::handle pbits, py
   if (how.history.defined()) {
     if (how.history.dim() != 2) refuse("history must be a tensor [rows, moves]");
     check_like(how.history, "history", logits, {at::kInt, at::kLong}, {rows, how.history.size(1)});
-    if (how.history.size(1) > (1 << 30)) refuse("history must have at most 2^30 moves a row");
+    if (how.history.size(1) > (1 << 28)) refuse("history must have at most 2^28 moves a row");
     if (!adjacent(how.history)) refuse("the entries of a row of history must lie next to each other");
   }
   if (how.history_len.defined()) {
