@@ -209,11 +209,17 @@ __device__ __forceinline__ void slab_sum(const NormCut& cut, int cpg, const Norm
   for (int j = 0; j < NV; ++j) lds[threadIdx.x * NV + j] = val[j];
   __syncthreads();
   const int mine = NV == 1 ? per : cpg;     // a group's values per row: they lie next to each other
+  const int down = 64 / mine, right = 64 - down * mine, row0 = lane / mine, col0 = lane - row0 * mine;
   for (int g = wave; g < cut.slab_groups; g += waves) {
     float v = 0.f;
-    for (int k = lane; k < cut.rows * mine; k += 64) {
-      const int row = k / mine;
-      v += lds[row * cut.units * NV + g * mine + (k - row * mine)];
+    for (int row = row0, col = col0; row < cut.rows;) {
+      v += lds[row * cut.units * NV + g * mine + col];
+      row += down;
+      col += right;
+      if (col >= mine) {
+        col -= mine;
+        ++row;
+      }
     }
     v = wave_sum(v);
     if (lane == 0) total[g] = v;
@@ -439,13 +445,28 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
           a1[j] += __shfl_xor(a1[j], d);
           a2[j] += __shfl_xor(a2[j], d);
         }
-    const int from = pow2 ? wave : q.row, many = pow2 ? waves : cut.rows;
-    if (pow2 ? lane < cut.units : q.on)
+    const int from = pow2 ? wave : q.row;
+    int many = pow2 ? waves : cut.rows;
+    auto put = [&](int at) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        red[(from * 2) * cut.width + q.unit * VEC + j] = a1[j];
-        red[(from * 2 + 1) * cut.width + q.unit * VEC + j] = a2[j];
+        red[(at * 2) * cut.width + q.unit * VEC + j] = a1[j];
+        red[(at * 2 + 1) * cut.width + q.unit * VEC + j] = a2[j];
       }
+    };
+    for (; many > 8 && !pow2; many -= many / 2) {   // rows in pairs, until eight are left
+      const int kept = many - many / 2;
+      if (q.on && from >= kept && from < many) put(from - kept);
+      __syncthreads();
+      if (q.on && from < many / 2)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          a1[j] += red[(from * 2) * cut.width + q.unit * VEC + j];
+          a2[j] += red[(from * 2 + 1) * cut.width + q.unit * VEC + j];
+        }
+      __syncthreads();
+    }
+    if (pow2 ? lane < cut.units : q.on && from < many) put(from);
     __syncthreads();
     for (int k = threadIdx.x; k < cut.width; k += blockDim.x) {
       float s1 = 0.f, s2 = 0.f;
@@ -460,16 +481,31 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
     }
     if (PHASE == NORM_SUMS) return;
   } else {
-    for (int k = threadIdx.x; k < cut.width; k += blockDim.x) {
+    // the chunks' sums of a channel, by as many threads as there are for it
+    const int each = (int)blockDim.x > cut.width ? (int)blockDim.x / cut.width : 1;
+    const float2* from = part + q.sample * cut.chunks * P.channels + q.c0;
+    for (int t = threadIdx.x; t < cut.width * each; t += blockDim.x) {
+      const int ch = t % cut.width;
       float s1 = 0.f, s2 = 0.f;
-      for (int i = 0; i < cut.chunks; ++i) {
-        const float2 v = part[(q.sample * cut.chunks + i) * P.channels + q.c0 + k];
+#pragma unroll 4
+      for (int i = t / cut.width; i < cut.chunks; i += each) {
+        const float2 v = from[(int64_t)i * P.channels + ch];
         s1 += v.x;
         s2 += v.y;
       }
-      const float wk = P.weight ? load_any(P.weight, P.param_dtype, q.c0 + k) : 1.f;
-      sum1[k] = wk * s1;
-      sum2[k] = wk * s2;
+      red[2 * t] = s1;
+      red[2 * t + 1] = s2;
+    }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < cut.width; ch += blockDim.x) {
+      float s1 = 0.f, s2 = 0.f;
+      for (int i = 0; i < each; ++i) {
+        s1 += red[2 * (i * cut.width + ch)];
+        s2 += red[2 * (i * cut.width + ch) + 1];
+      }
+      const float wk = P.weight ? load_any(P.weight, P.param_dtype, q.c0 + ch) : 1.f;
+      sum1[ch] = wk * s1;
+      sum2[ch] = wk * s2;
     }
   }
   __syncthreads();
@@ -1101,37 +1137,58 @@ struct NormPlan {
 NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int dtype, bool residual, bool grad, int vec = 0) {
   NormPlan p;
   const int cpg = channels / groups, widest = norm_vec(channels, dtype), size = dtype == GOENV_DT_F32 ? 4 : 2;
-  // Slabs: as narrow as whole groups and vectors allow, but 64 bytes of a position where that leaves 512 workgroups (2,048 boards
-  // of 128 bf16 channels in 8 groups: 32 bytes 150 us, 64 bytes 123 us, 128 bytes 134 us).
-  auto next_of = [&](int gs) {
-    do ++gs;
-    while (gs <= groups && (groups % gs || (gs * cpg) % widest));
-    return gs;
-  };
-  int gs = next_of(0);
-  while (gs < groups && gs * cpg * size < 64 && n * (groups / next_of(gs)) >= 512) gs = next_of(gs);
-  // Threads: few vectors each while there are few workgroups, six where there are many.
-  auto vectors_at = [&](int threads, int64_t of) {
+  // Slabs are whole groups and whole vectors.  Wide ones: full cache lines of a position (128 bytes) where up to 384 bytes give them,
+  // else up to 320 bytes (2,048 boards of 128 bf16 channels in 8 groups: 32 bytes 150 us, 64 bytes 124 us, 128 bytes
+  // 124 us and the gradient 236 / 227 us; 378 boards of 240 channels in 24 groups: 80 bytes 51 us, 240 bytes 39 us).
+  auto fits = [&](int gs) { return groups % gs == 0 && (gs * cpg) % widest == 0; };
+  int least = 1;
+  while (!fits(least)) ++least;
+  int gs = least;
+  for (int i = least; i <= groups && i * cpg * size <= 384; ++i) {
+    if (!fits(i) || (i * cpg * size > 320 && (i * cpg * size) % 128)) continue;
+    gs = i;
+    if ((i * cpg * size) % 128 == 0) break;
+  }
+  auto vectors_at = [&](int threads, int64_t of) {   // of a thread
     const int rows = threads / (gs * cpg / widest);
     return rows ? (of + rows - 1) / rows : of;
   };
-  auto threads_for = [&](int64_t of, int most) {
-    int t = 64;
-    while (t < NORM_THREADS && (t < gs * cpg / widest || vectors_at(t, of) > most)) t *= 2;
-    return t;
+  // Fewer workgroups than CUs: slabs get narrower, to half lines at first.  If that leaves them too few or too long, the axis is cut
+  // into chunks of eight vectors a thread instead (64 x 100 x 100 positions of 64 bf16 channels: 134 -> 66 us, 250 -> 139 us;
+  // two images of 128 x 128 x 256 56 -> 16, 81 -> 26 us).  A few thousand workgroups take half lines too: the last
+  // round of them counts (256 boards of 128 float32 channels: 36 -> 30 us, 66 -> 59 us).
+  auto narrower = [&](int gs, int bytes) {   // the next one that is not below `bytes`, or the same
+    for (int i = gs - 1; i >= least && i * cpg * size >= bytes; --i)
+      if (fits(i)) return i;
+    return gs;
   };
-  const int64_t wgs = n * (groups / gs);
-  p.threads = threads_for(positions, wgs < 64 ? 2 : wgs < 512 ? 3 : 6);
-  // A long axis with few workgroups is cut into chunks of `part` vectors a thread, at most `many`.
+  auto wgs_of = [&](int gs) { return n * (groups / gs); };
   int64_t chunks = 1;
-  const int part = grad ? 8 : 4, many = grad ? 32 : 64;
-  if (wgs < 256 && vectors_at(NORM_THREADS, positions) > 12) {
-    while (gs < groups && gs * cpg * size < (grad ? 64 : 128)) gs = next_of(gs);
-    p.threads = NORM_THREADS;
-    chunks = (vectors_at(p.threads, positions) + part - 1) / part;
-    if (chunks > many) chunks = many;
+  if (wgs_of(gs) < 256) {
+    const int wide = gs;
+    while (wgs_of(gs) < 256 && narrower(gs, 64) != gs) gs = narrower(gs, 64);
+    const int64_t v = vectors_at(NORM_THREADS, positions);
+    if (v > (wgs_of(gs) < 256 ? 12 : 16)) {
+      gs = wide;
+      chunks = (vectors_at(NORM_THREADS, positions) + 7) / 8;
+      const int64_t most = (2047 + wgs_of(gs)) / wgs_of(gs);
+      if (chunks > most) chunks = most;
+    } else {
+      while (wgs_of(gs) < 256 && narrower(gs, 1) != gs) gs = narrower(gs, 1);
+    }
+  } else if (wgs_of(gs) < 2048 && gs * cpg * size % 128 == 0) {
+    for (int i = least; i < gs; ++i)
+      if (fits(i) && i * cpg * size == 64) gs = i;
   }
-  const int most = (grad ? 32 : 48) << 10;
+  // As many threads as leave each a few vectors: six where there are many workgroups, but three in the forward pass while a vector lies
+  // in one group (else the sums over a slab grow with the threads).  LDS for three workgroups of 512 threads on a CU, five
+  // (forward) or four smaller ones (256 boards of 128 bf16 channels, forward: 512 threads 15.5 us, 256 threads 16.0; of float32
+  // 30 / 40 us; the gradient in bf16 with 256 threads: 52 KB 34 us, 40 KB 28 us, with 512 31 us).
+  const int64_t of = (positions + chunks - 1) / chunks, wgs = wgs_of(gs) * chunks;
+  const int few = wgs < 64 ? 2 : wgs < 512 || (!grad && cpg % widest == 0) ? 3 : 6;
+  p.threads = 64;
+  while (p.threads < NORM_THREADS && (p.threads < gs * cpg / widest || vectors_at(p.threads, of) > few)) p.threads *= 2;
+  const int most = p.threads == NORM_THREADS ? 52 << 10 : grad ? 40 << 10 : 32 << 10;
   NormCut& c = p.cut;
   p.vec = vec ? vec : widest;
   c.slab_groups = gs;
@@ -1144,14 +1201,16 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   p.split = c.chunks > 1;
   if (c.rows == 0) return p;
   if (grad) {
-    const int parts = c.units <= 64 && (c.units & (c.units - 1)) == 0 ? p.threads / 64 : c.rows;
-    c.scratch = 2 * c.width + 2 * gs + 2 * parts * c.width;
+    const int parts = c.units <= 64 && (c.units & (c.units - 1)) == 0 ? p.threads / 64 : c.rows <= 8 ? c.rows : c.rows / 2 > 8 ? c.rows / 2 : 8;
+    const int sums = parts * c.width;
+    c.scratch = 2 * c.width + 2 * gs + 2 * (sums > p.threads ? sums : p.threads);
   } else {
     c.scratch = p.threads * (cpg % p.vec == 0 ? 1 : p.vec) + 2 * gs;
   }
   c.scratch = (c.scratch + 3) & ~3;
   const int64_t vectors = (c.chunk + c.rows - 1) / c.rows, row = (int64_t)p.threads * p.vec * size * (1 + grad + residual);
-  c.staged = (int)(vectors < most / row ? vectors : most / row);
+  const int64_t room = most > c.scratch * 4 ? (most - c.scratch * 4) / row : 0;
+  c.staged = (int)(vectors < room ? vectors : room);
   p.lds = c.scratch * sizeof(float) + c.staged * row;
   return p;
 }
