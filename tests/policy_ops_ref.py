@@ -108,8 +108,9 @@ def threshold(p):
     return int(math.floor(p * 65536 + 0.5))
 
 
-def keep_mask(n, seed, step, site, p):
-    blk = np.arange((n + 7) // 8, dtype=np.uint64)
+def keep_mask(n, seed, step, site, p, first=0):
+    """Of n elements from block `first` on."""
+    blk = np.arange(first, first + (n + 7) // 8, dtype=np.uint64)
     words = philox((blk & np.uint64(0xFFFFFFFF), blk >> np.uint64(32), np.full_like(blk, step & 0xFFFFFFFF),
                     np.full_like(blk, site)), (seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF))
     bits = [w & np.uint64(0xFFFF) for w in words] + [w >> np.uint64(16) for w in words]

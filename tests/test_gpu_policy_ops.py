@@ -61,6 +61,12 @@ NORM = [
     (1, 16, 8, (200, 201), F16, "silu", False, F32),
     (1, 7, 1, (150, 151), F32, "none", True, F32),
     (300, 24, 6, (2, 2), BF16, "leaky_relu", False, F32),
+    (2, 5000, 1, (3,), BF16, "leaky_relu", True, F32),          # groups wider than a workgroup's vectors
+    (2, 1025, 1, (5,), F32, "silu", False, F32),
+    (130, 96, 32, (25, 25), F16, "relu", True, F32),
+    (40, 15, 5, (23, 9), BF16, "silu", True, F32),
+    (3, 240, 24, (50, 51), BF16, "leaky_relu", True, F32),
+    (2, 128, 128, (40, 41), F32, "none", False, F32),
 ]
 ids = lambda v: str(v).replace("torch.", "").replace(" ", "")                             # noqa: E731
 
@@ -216,7 +222,33 @@ def test_group_norm_refusals(ops, error):
             call()
 
 
+def test_group_norm_beyond_32_bit_offsets(ops):
+    """The last samples of a tensor of 2.3 billion elements, forward and backward, against themselves alone (a sample's result
+    does not depend on the others; the launch shapes differ, so within a rounding of the type)."""
+    n, c = 50000, 128
+    x = torch.randn(64, 19 * 19, c, device="cuda").to(BF16).repeat(n // 64 + 1, 1, 1)[:n]
+    x[-3:] = torch.randn(3, 19 * 19, c, device="cuda").to(BF16)
+    x = x.movedim(-1, 1).requires_grad_(True)
+    y = ops.group_norm_act(x, 8, act="leaky_relu")
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    tail = x.detach()[-3:].clone(memory_format=torch.preserve_format)
+    want = ref.group_norm_act(tail, 8, None, None, 1e-5, "leaky_relu", 0.1, None, tail)
+    assert_within(y[-3:], want["y"])
+    assert_within(dx[-3:], want["dx"])
+
+
 # ---- dropout ----------------------------------------------------------------------------------------------------
+def test_dropout_beyond_32_bit_offsets(ops):
+    """The last elements of 2^32 + 13: the block counter's high word takes part from 2^35 elements on, offsets from 2^31."""
+    n = (1 << 32) + 13
+    x = torch.ones(n, dtype=BF16, device="cuda")
+    y = ops.dropout(x, 0.5, rng_of(5, 6), 7)[-2061:].cpu()
+    first = n - 2061
+    assert first % 8 == 0
+    kept = ref.keep_mask(2061, 5, 6, 7, 0.5, first // 8)
+    assert torch.equal(y != 0, kept) and bool((y[kept] == 2).all())
+
+
 def rng_of(seed, step):
     return torch.tensor([seed, step], dtype=torch.int64, device="cuda")
 
@@ -500,6 +532,21 @@ def test_policy_logits_gradients_against_differences(ops, cols, out):
         formula, formula64 = (float((wide(d) * wide(way)).sum()) for d in (got[k], want["d" + k][0]))
         spare += float((want["d" + k][1] * wide(way).abs()).sum())
         assert abs(slope - formula) <= abs(slope64 - formula64) + spare, k
+
+
+def test_policy_logits_beyond_32_bit_offsets(ops):
+    """The last rows of 2.3 billion logits, forward and backward."""
+    rows, cols = 6_300_000, 361
+    x = torch.randn(64, cols, device="cuda").to(BF16).repeat(rows // 64 + 1, 1)[:rows]
+    x[-2:] = torch.randn(2, cols, device="cuda").to(BF16)
+    legal = (torch.arange(cols, device="cuda") % 3 > 0).expand(rows, cols)
+    x.requires_grad_(True)
+    y = ops.policy_logits(x, legal=legal, out="log_probs")
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    tail = x.detach()[-2:]
+    want = ref.policy_logits(tail, legal[-2:], out="log_probs", dy=tail)
+    assert_within(y[-2:], want["y"])
+    assert_within(dx[-2:], want["dlogits"])
 
 
 def test_policy_logits_empty(ops):

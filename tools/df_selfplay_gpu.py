@@ -52,17 +52,22 @@ def main():
     ap.add_argument("--num_block", type=int, default=20)
     ap.add_argument("--dim", type=int, default=128)
     ap.add_argument("--bf16", action="store_true")
+    ap.add_argument("--groups", type=int, default=0, help="group norm with that many groups instead of BatchNorm")
+    ap.add_argument("--mask_policy", action="store_true", help="the net's pi is taken over the legal points")
+    ap.add_argument("--temperature", type=float, default=1.0, help="of the policy's logits")
     ap.add_argument("--json", action="store_true", help="rank 0 prints a JSON line instead of text")
     ap.set_defaults(mode="selfplay", num_games=4096, batchsize=1024, num_collectors=0, seed=1, ply_cap=722,
                     end_on_two_passes=True, signal_restart=True)
     args = ap.parse_args()
     args.gpu = local_rank if world > 1 or args.gpu is None else args.gpu
     args.board_id_base = rank * args.num_games
+    args.legal_mask = args.legal_mask or args.mask_policy
     torch.cuda.set_device(args.gpu)
     GC = go_loader.initialize(args)
     dev = torch.device("cuda", args.gpu)
     torch.manual_seed(1)                      # every rank builds the same random-initialised actor
-    net = PolicyValueNet(dim=args.dim, num_block=args.num_block).to(dev).eval()
+    net = PolicyValueNet(dim=args.dim, num_block=args.num_block, norm="group" if args.groups else "batch",
+                         groups=args.groups).to(dev).eval()
     if args.bf16:
         net = net.to(torch.bfloat16).to(memory_format=torch.channels_last)
     t_model = [0.0]
@@ -70,8 +75,9 @@ def main():
 
     def actor(batch):
         ev0.record()
+        b = batch.hist(0)
         with torch.no_grad():
-            out = net(batch.hist(0))
+            out = net(b, b["legal"] if args.mask_policy else None, args.temperature)
         ev1.record()
         ev1.synchronize()
         t_model[0] += ev0.elapsed_time(ev1) * 1e-3

@@ -20,19 +20,30 @@ import torch  # noqa: E402
 import torch.nn as nn  # noqa: E402
 import torch.nn.functional as F  # noqa: E402
 
-from elf_amd import go_loader  # noqa: E402
+from elf_amd import go_loader, policy_ops  # noqa: E402
 
 
 class PolicyNet(nn.Module):
-    def __init__(self, planes=25, dim=128, layers=39, k=3):
+    def __init__(self, planes=25, dim=128, layers=39, k=3, groups=0, dropout=0.0):
         super().__init__()
+        self.groups, self.dropout = groups, dropout
         self.convs = nn.ModuleList([nn.Conv2d(planes if i == 0 else dim, dim, 3, padding=1) for i in range(layers)])
-        self.bns = nn.ModuleList([nn.BatchNorm2d(dim) for _ in range(layers)])
+        if groups:                                 # conv -> norm -> activation, one kernel behind the convolution
+            self.norms = nn.ModuleList([policy_ops.GroupNormAct(groups, dim, act="leaky_relu") for _ in range(layers)])
+        else:
+            self.bns = nn.ModuleList([nn.BatchNorm2d(dim) for _ in range(layers)])
+        self.state = policy_ops.DropoutState(seed=1) if dropout else None
         self.final = nn.Conv2d(dim, k, 3, padding=1)
 
     def forward(self, s):
-        for conv, bn in zip(self.convs, self.bns):
-            s = bn(F.leaky_relu(conv(s), 0.1))
+        if self.groups:
+            for conv, norm in zip(self.convs, self.norms):
+                s = norm(conv(s).contiguous(memory_format=torch.channels_last))
+        else:
+            for conv, bn in zip(self.convs, self.bns):
+                s = bn(F.leaky_relu(conv(s), 0.1))
+        if self.dropout and self.training:
+            s = policy_ops.dropout(s, self.dropout, self.state.rng)
         return self.final(s).flatten(2)            # [B, k, 361] logits
 
 
@@ -42,6 +53,9 @@ def main():
     ap.add_argument("--num_layer", type=int, default=39)
     ap.add_argument("--dim", type=int, default=128)
     ap.add_argument("--bf16", action="store_true")
+    ap.add_argument("--groups", type=int, default=0, help="group norm with that many groups instead of BatchNorm")
+    ap.add_argument("--dropout", type=float, default=0.0, help="dropout in front of the last convolution")
+    ap.add_argument("--fused_loss", action="store_true", help="log probabilities through policy_ops.policy_logits")
     ap.add_argument("--lr", type=float, default=0.01)
     ap.set_defaults(mode="offline", gpu=0, num_games=256, batchsize=256, num_collectors=1, seed=7, T=1,
                     num_games_per_thread=300, list_file=os.path.join(ROOT, "tests", "golden", "corpus", "train.lst"))
@@ -49,8 +63,8 @@ def main():
     GC = go_loader.initialize(args)
     dev = torch.device("cuda", args.gpu)
     k = args.num_future_actions
-    net = PolicyNet(dim=args.dim, layers=args.num_layer, k=k).to(dev).train()
-    if args.bf16:
+    net = PolicyNet(dim=args.dim, layers=args.num_layer, k=k, groups=args.groups, dropout=args.dropout).to(dev).train()
+    if args.bf16 or args.groups:
         net = net.to(memory_format=torch.channels_last)
     opt = torch.optim.SGD(net.parameters(), lr=args.lr, momentum=0.9)
     t_model, losses = [0.0], []
@@ -62,10 +76,16 @@ def main():
         ev0.record()
         with torch.autocast("cuda", dtype=torch.bfloat16, enabled=args.bf16):
             logits = net(s)
-        loss = sum(F.cross_entropy(logits[:, i].float(), target[:, i]) for i in range(k))
+        if args.fused_loss:
+            logp = policy_ops.policy_logits(logits.reshape(-1, logits.shape[2]), out="log_probs", dtype=torch.float32)
+            loss = k * F.nll_loss(logp, target[:, :k].reshape(-1))
+        else:
+            loss = sum(F.cross_entropy(logits[:, i].float(), target[:, i]) for i in range(k))
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()
+        if net.state is not None:
+            net.state.advance()
         ev1.record()
         ev1.synchronize()
         t_model[0] += ev0.elapsed_time(ev1) * 1e-3
