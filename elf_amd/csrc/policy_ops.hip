@@ -775,6 +775,12 @@ enum LogitMode { LOGIT_MAP, LOGIT_WHOLE, LOGIT_SUMS, LOGIT_APPLY };   // no soft
 struct RowRules {
   float inv_rep, rep, presence, frequency, inv_t;
 };
+// A scalar argument as a register's value: left as a place in memory, the choice between it and a row's value becomes a choice between
+// two addresses, and the arguments are copied to the stack for it.
+__device__ __forceinline__ float in_register(float v) {
+  asm("" : "+s"(v));
+  return v;
+}
 __device__ __forceinline__ RowRules rules_of(const goenv_logit_rules& P, int64_t row) {
   RowRules r;
   float t;
@@ -784,10 +790,14 @@ __device__ __forceinline__ RowRules rules_of(const goenv_logit_rules& P, int64_t
     r.frequency = P.row_frequency[row];
     t = P.row_temperature[row];
   } else {
-    r.rep = P.row_repetition ? P.row_repetition[row] : P.repetition;
-    r.presence = P.row_presence ? P.row_presence[row] : P.presence;
-    r.frequency = P.row_frequency ? P.row_frequency[row] : P.frequency;
-    t = P.row_temperature ? P.row_temperature[row] : P.temperature;
+    r.rep = in_register(P.repetition);
+    r.presence = in_register(P.presence);
+    r.frequency = in_register(P.frequency);
+    t = in_register(P.temperature);
+    if (P.row_repetition) r.rep = P.row_repetition[row];
+    if (P.row_presence) r.presence = P.row_presence[row];
+    if (P.row_frequency) r.frequency = P.row_frequency[row];
+    if (P.row_temperature) t = P.row_temperature[row];
   }
   r.inv_rep = 1.f / r.rep;
   r.inv_t = 1.f / t;
@@ -832,12 +842,14 @@ __device__ __forceinline__ void store_columns(void* p, bool f32, int64_t at, con
   else store_row<T, VEC, NI>(static_cast<T*>(p) + at, col, in, from);
 }
 
-// This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end), and dz / dlogit without the
-// temperature; returns 1 / temperature.  count: LDS, a word per column of the slice; every thread of the team calls.
+// This thread's columns of a slice of a row: z (-inf where it is off or behind the row's end); in `seen` and `up` a bit per column,
+// whether it stands in the history and whether its logit is above zero (what dz / dlogit goes by); returns the
+// row's rules.  count: LDS, a word per column of the slice; every thread of the team calls.  have_bias: `bias` is loaded already.
 // All loads start before anything waits for one: a short row's time is the time of its longest chain of loads.
 template <typename T, int VEC, int NI, bool WAVE>
-__device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, int64_t row, uint32_t v0, const uint32_t (&col)[NI],
-                                          const bool (&in)[NI], int* count, float (&z)[NI][VEC], float (&slope)[NI][VEC]) {
+__device__ __forceinline__ RowRules slice_of(const goenv_logit_rules& P, const Team<WAVE>& team, int64_t row, uint32_t v0, const uint32_t (&col)[NI],
+                                             const bool (&in)[NI], int* count, float (&z)[NI][VEC], uint32_t& seen, uint32_t& up, bool have_bias,
+                                             float (&bias)[NI][VEC]) {
   const T* logits = static_cast<const T*>(P.logits) + row * P.logits_row;
   Pack<T, VEC> raw[NI];
 #pragma unroll
@@ -852,8 +864,8 @@ __device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team
 #pragma unroll
     for (int k = 0; k < NI; ++k) mask[k] = *in_row<const uint32_t>(bits, (col[k] >> 5) * 4);
   }
-  float bias[NI][VEC];
-  if (P.bias) load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, row * P.bias_row, col, bias);
+  if (P.bias && !have_bias) load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, row * P.bias_row, col, bias);
+  seen = up = 0;
   const bool past = P.history && P.history_max > 0;
   const uint32_t width = (uint32_t)(NI * VEC * team.threads), left = (uint32_t)P.cols - v0, most = width < left ? width : left;
   RowRules r;
@@ -898,7 +910,8 @@ __device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team
       for (int j = 0; j < VEC; ++j) {
         const int c = count[(k * team.threads + team.tid) * VEC + j];
         const float l = (float)raw[k].v[j], f = l > 0.f ? r.inv_rep : r.rep;
-        slope[k][j] = c > 0 ? f : 1.f;
+        seen |= (uint32_t)(c > 0) << (k * VEC + j);
+        up |= (uint32_t)(l > 0.f) << (k * VEC + j);
         z[k][j] = c > 0 ? l * f - r.presence - r.frequency * (float)c : l;
       }
   } else {
@@ -906,10 +919,7 @@ __device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        slope[k][j] = 1.f;
-        z[k][j] = (float)raw[k].v[j];
-      }
+      for (int j = 0; j < VEC; ++j) z[k][j] = (float)raw[k].v[j];
   }
   if (P.bias)
 #pragma unroll
@@ -925,7 +935,7 @@ __device__ __forceinline__ float slice_of(const goenv_logit_rules& P, const Team
   if (P.legal) finish([&](int k, int j) { return (mask[k] & (0xffu << (8 * j))) != 0; });
   else if (P.legal_bits) finish([&](int k, int j) { return ((mask[k] >> ((col[k] + j) & 31)) & 1u) != 0; });
   else finish([](int, int) { return true; });
-  return r.inv_t;
+  return r;
 }
 
 template <int VEC, int NI, bool WAVE>
@@ -952,8 +962,9 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
   uint32_t col[NI];
   bool in[NI];
   columns_of<VEC, NI>(P, team, v0, col, in);
-  float z[NI][VEC], slope[NI][VEC];
-  slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, slope);
+  float z[NI][VEC], bias[NI][VEC];
+  uint32_t seen, up;
+  slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, seen, up, false, bias);
   if (MODE != LOGIT_MAP) {
     float m = -INFINITY, s = 0.f;
     if (MODE != LOGIT_APPLY) {
@@ -1004,9 +1015,10 @@ __global__ __launch_bounds__(1024) void k_policy_logits(goenv_logit_rules P, Log
   store_columns<T, VEC, NI>(out, P.out_dtype == GOENV_DT_F32, row * P.cols, col, in, z);
 }
 
-// The gradients.  The workspace: a row's slices' sums of dy (log probabilities) or p dy (probabilities), then the row groups'
-// sums of dz for a bias that all rows share.
-template <typename T, int VEC, int NI, bool WAVE, int MODE>
+// The gradients.  SHARED: of a bias that all rows share too -- a workgroup then takes several rows one after the other and
+// keeps the sums of dz.  The workspace: a row's slices' sums of dy (log probabilities) or p dy (probabilities), then the
+// row groups' sums of dz.
+template <typename T, int VEC, int NI, bool WAVE, bool SHARED, int MODE>
 __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P, LogitCut cut, const void* d_out, int64_t dy_row, T* dlogits,
                                                              void* dbias, float* shared) {
   extern __shared__ __align__(16) int counts[];
@@ -1020,16 +1032,21 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
   uint32_t col[NI];
   bool in[NI];
   columns_of<VEC, NI>(P, team, v0, col, in);
-  float sum[NI][VEC];
+  float sum[SHARED ? NI : 1][VEC], bias[NI][VEC];
+  if (SHARED) {
 #pragma unroll
-  for (int k = 0; k < NI; ++k)
+    for (int k = 0; k < NI; ++k)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[k][j] = 0.f;
-  const int64_t end = (group + 1) * cut.per_group < P.rows ? (group + 1) * cut.per_group : P.rows;
-  for (int64_t row = group * cut.per_group; row < end; ++row) {
-    float z[NI][VEC], slope[NI][VEC], dz[NI][VEC];
+      for (int j = 0; j < VEC; ++j) sum[k][j] = 0.f;
+    load_columns<T, VEC, NI>(P.bias, P.bias_dtype == GOENV_DT_F32, 0, col, bias);
+  }
+  const int64_t first = SHARED ? group * cut.per_group : group;
+  const int64_t end = !SHARED ? first + 1 : first + cut.per_group < P.rows ? first + cut.per_group : P.rows;
+  for (int64_t row = first; row < end; ++row) {
+    float z[NI][VEC], dz[NI][VEC];
+    uint32_t seen, up;
     load_columns<T, VEC, NI>(d_out, P.out_dtype == GOENV_DT_F32, row * dy_row, col, dz);
-    const float inv_t = slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, slope);
+    const RowRules r = slice_of<T, VEC, NI>(P, team, row, v0, col, in, count, z, seen, up, SHARED, bias);
     if (MODE != LOGIT_MAP) {
       const float m = P.stats[2 * row], inv_s = 1.f / P.stats[2 * row + 1];
       const bool probs = P.out_kind == GOENV_OUT_PROBS;
@@ -1038,48 +1055,71 @@ __global__ __launch_bounds__(1024) void k_policy_logits_grad(goenv_logit_rules P
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
+        for (int j = 0; j < VEC; ++j) {   // z becomes p
           const bool off = z[k][j] == -INFINITY;
-          const float p = __expf(z[k][j] - m) * inv_s;
-          slope[k][j] = off ? 0.f : slope[k][j];
           dz[k][j] = off ? 0.f : dz[k][j];
-          z[k][j] = off ? 0.f : p;
-          total += probs ? z[k][j] * dz[k][j] : dz[k][j];
+          z[k][j] = off ? 0.f : __expf(z[k][j] - m) * inv_s;
         }
-      if (MODE == LOGIT_APPLY) {
-        total = 0.f;
+      if (MODE != LOGIT_APPLY) {
+        if (probs) {
+#pragma unroll
+          for (int k = 0; k < NI; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) total += z[k][j] * dz[k][j];
+        } else {
+#pragma unroll
+          for (int k = 0; k < NI; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) total += dz[k][j];
+        }
+        total = team.sum(total, lds);
+      } else {
         for (int k = threadIdx.x & 63; k < cut.slices; k += 64) total += part[k];
         total = wave_sum(total);
-      } else {
-        total = team.sum(total, lds);
       }
       if (MODE == LOGIT_SUMS) {
         if (team.tid == 0) part[slice] = total;
         continue;
       }
+      if (probs) {
+#pragma unroll
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) dz[k][j] = z[k][j] * (dz[k][j] - total);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) dz[k][j] -= z[k][j] * total;
+      }
+    } else {
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) dz[k][j] = probs ? z[k][j] * (dz[k][j] - total) : dz[k][j] - z[k][j] * total;
+        for (int j = 0; j < VEC; ++j) dz[k][j] = z[k][j] == -INFINITY ? 0.f : dz[k][j];
     }
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        if (MODE == LOGIT_MAP && z[k][j] == -INFINITY) dz[k][j] = slope[k][j] = 0.f;
-        dz[k][j] *= inv_t;
-        sum[k][j] += dz[k][j];
+        dz[k][j] *= r.inv_t;
+        if (SHARED) sum[k][j] += dz[k][j];
       }
-    if (dbias && !shared) store_columns<T, VEC, NI>(dbias, P.bias_dtype == GOENV_DT_F32, row * P.cols, col, in, dz);
+    if (dbias && !SHARED) store_columns<T, VEC, NI>(dbias, P.bias_dtype == GOENV_DT_F32, row * P.cols, col, in, dz);
     if (dlogits) {
+      if (seen)
 #pragma unroll
-      for (int k = 0; k < NI; ++k)
+        for (int k = 0; k < NI; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) dz[k][j] *= slope[k][j];
+          for (int j = 0; j < VEC; ++j) {
+            const uint32_t bit = 1u << (k * VEC + j);
+            if (dz[k][j] != 0.f) dz[k][j] *= (seen & bit) == 0 ? 1.f : (up & bit) ? r.inv_rep : r.rep;   // (0 stays 0 whatever the factor)
+          }
       store_columns<T, VEC, NI>(dlogits, sizeof(T) == 4, row * P.cols, col, in, dz);
     }
   }
-  if (MODE != LOGIT_SUMS && shared) store_columns<float, VEC, NI>(shared, true, group * P.cols, col, in, sum);
+  if constexpr (SHARED)
+    if (MODE != LOGIT_SUMS) store_columns<float, VEC, NI>(shared, true, group * P.cols, col, in, sum);
 }
 
 // Column sums of [rows][cols], 16 columns (half a cache line) a workgroup, 64 rows at a time
@@ -1245,12 +1285,11 @@ struct LogitPlan {
   unsigned blocks(int64_t teams) const { return (unsigned)(wave ? (teams + 3) / 4 : teams); }
 };
 
-// The cut for vectors of `vec` columns (which goes by the arrays' alignment: a workspace is sized for either).  The gradient holds four
-// values a column, twice what the forward pass holds.
-LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, bool grad, int vec) {
+// The cut for vectors of `vec` columns (which goes by the arrays' alignment: a workspace is sized for either).  
+LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, int vec) {
   LogitPlan p;
   p.vec = vec;
-  p.ni = vec == 1 ? 6 : grad ? 2 : 4;
+  p.ni = vec == 1 ? 6 : shared ? 2 : 4;   // (the sums of a shared bias's gradient and the bias itself are in registers too)
   const int each = p.ni * vec;             // columns of a thread
   p.split = softmax && cols > 1024 * each;
   p.threads = 64;
@@ -1261,8 +1300,9 @@ LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, bool
   p.cut.slices = (int)((cols + (int64_t)p.cut.threads * each - 1) / ((int64_t)p.cut.threads * each));
   p.cut.per_group = 1;
   if (shared) {
-    const int64_t wgs = rows * p.cut.slices, most = rows < 65536 ? rows : 65536;
-    p.cut.per_group = (int)(wgs <= 1024 ? 1 : (wgs + 1023) / 1024 < most ? (wgs + 1023) / 1024 : most);
+    // no more rows in a group than leave half a million threads at work
+    const int64_t teams = rows * p.cut.slices, want = (1 << 19) / p.cut.threads, per = (teams + want - 1) / want;
+    p.cut.per_group = (int)(per < 1 ? 1 : per > rows ? rows : per);
   }
   p.cut.groups = (rows + p.cut.per_group - 1) / p.cut.per_group;
   return p;
@@ -1467,7 +1507,7 @@ int64_t goenv_policy_logits_workspace(int64_t rows, int64_t cols, int out_kind, 
   const bool softmax = out_kind != GOENV_OUT_LOGITS;
   int64_t most = 0;
   for (int vec : {1, 4}) {
-    const LogitPlan p = logit_plan(rows, cols, softmax, grad && shared_bias, grad, vec);
+    const LogitPlan p = logit_plan(rows, cols, softmax, grad && shared_bias, vec);
     int64_t need = p.split ? rows * p.cut.slices * (int64_t)(grad ? sizeof(float) : sizeof(float2)) : 0;
     if (grad && shared_bias) need = ((need + 15) & ~15) + p.cut.groups * cols * (int64_t)sizeof(float);
     most = need > most ? need : most;
@@ -1480,7 +1520,7 @@ int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream) {
   if (p->rows == 0 || p->cols == 0) return 0;
   if (!out || !aligned(out, p->out_dtype)) return fail("goenv_policy_logits: out is required, aligned to its elements");
   const bool softmax = p->out_kind != GOENV_OUT_LOGITS;
-  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, false, false, logit_fours(p, nullptr, 0, out, p->out_dtype, nullptr, 0) ? 4 : 1);
+  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, false, logit_fours(p, nullptr, 0, out, p->out_dtype, nullptr, 0) ? 4 : 1);
   if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits");
   by_dtype(p->dtype, [&](auto t) {
@@ -1513,7 +1553,7 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
   const bool shared = dbias && p->bias_row == 0, softmax = p->out_kind != GOENV_OUT_LOGITS;
   if (p->rows > 0 && (!d_out || !aligned(d_out, p->out_dtype) || !aligned(dlogits, p->dtype) || !aligned(dbias, p->bias_dtype)))
     return fail("goenv_policy_logits_grad: d_out is required, and the arrays aligned to their elements");
-  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, shared, true,
+  const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, shared,
                                     logit_fours(p, d_out, dy_row, dlogits, p->dtype, shared ? nullptr : dbias, p->bias_dtype) ? 4 : 1);
   if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits_grad: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits_grad");
@@ -1522,23 +1562,29 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
   if (p->rows > 0) {
     by_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
-      auto with = [&](auto v, auto n) {
+      auto with = [&](auto v, auto n, auto b) {
         constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
+        constexpr bool SHARED = decltype(b)::value;
         const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
         auto go = [&](auto f) {
           hipLaunchKernelGGL(f, dim3(plan.blocks(plan.cut.groups * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, d_out,
                              dy_row, static_cast<T*>(dlogits), dbias, parts);
         };
-        if (!softmax) {
-          plan.wave ? go(k_policy_logits_grad<T, VEC, NI, true, LOGIT_MAP>) : go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_MAP>);
-        } else if (!plan.split) {
-          plan.wave ? go(k_policy_logits_grad<T, VEC, NI, true, LOGIT_WHOLE>) : go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_WHOLE>);
-        } else {
-          go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_SUMS>);
-          go(k_policy_logits_grad<T, VEC, NI, false, LOGIT_APPLY>);
-        }
+        auto launch = [&](auto w) {
+          constexpr bool WAVE = decltype(w)::value;
+          if (!softmax) {
+            go(k_policy_logits_grad<T, VEC, NI, WAVE, SHARED, LOGIT_MAP>);
+          } else if (!plan.split) {
+            go(k_policy_logits_grad<T, VEC, NI, WAVE, SHARED, LOGIT_WHOLE>);
+          } else if constexpr (!WAVE) {
+            go(k_policy_logits_grad<T, VEC, NI, WAVE, SHARED, LOGIT_SUMS>);
+            go(k_policy_logits_grad<T, VEC, NI, WAVE, SHARED, LOGIT_APPLY>);
+          }
+        };
+        plan.wave ? launch(Int<1>()) : launch(Int<0>());
       };
-      plan.vec == 4 ? with(Int<4>(), Int<2>()) : with(Int<1>(), Int<6>());
+      if (plan.vec == 4) shared ? with(Int<4>(), Int<2>(), Int<1>()) : with(Int<4>(), Int<4>(), Int<0>());
+      else shared ? with(Int<1>(), Int<6>(), Int<1>()) : with(Int<1>(), Int<6>(), Int<0>());
     });
     HIPCHK(hipGetLastError());
   }
