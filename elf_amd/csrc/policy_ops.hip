@@ -178,7 +178,7 @@ __device__ __forceinline__ NormPlace norm_place(const goenv_norm& P, const NormC
   return q;
 }
 
-__device__ __forceinline__ bool is_pow2(int v) { return (v & (v - 1)) == 0; }
+__host__ __device__ __forceinline__ bool is_pow2(int v) { return (v & (v - 1)) == 0; }
 
 // Sums over a slab's groups.  Each thread brings its vector's sum: NV = 1 where a vector lies within one group, else a value per
 // channel.  Where the vectors of a position and of a group are powers of two that fit a wave, lanes are added up by
@@ -1195,8 +1195,10 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   };
   // Fewer workgroups than CUs: slabs get narrower, to half lines at first.  If that leaves them too few or too long, the axis is cut
   // into chunks of eight vectors a thread instead (64 x 100 x 100 positions of 64 bf16 channels: 134 -> 66 us, 250 -> 139 us;
-  // two images of 128 x 128 x 256 56 -> 16, 81 -> 26 us).  A few thousand workgroups take half lines too: the last
-  // round of them counts (256 boards of 128 float32 channels: 36 -> 30 us, 66 -> 59 us).
+  // two images of 128 x 128 x 256 56 -> 16, 81 -> 26 us).  Half lines are as good while the slab is staged whole,
+  // and keep the last round of workgroups short: the forward pass takes them, the gradient while it has few workgroups (512 boards
+  // of 256 bf16 channels, forward: 70 us with lines, 67 with half lines; 2,048 boards of 128, the gradient: 227 and 238; 256
+  // boards of 128 float32 channels, the gradient: 62 and 57).
   auto narrower = [&](int gs, int bytes) {   // the next one that is not below `bytes`, or the same
     for (int i = gs - 1; i >= least && i * cpg * size >= bytes; --i)
       if (fits(i)) return i;
@@ -1216,19 +1218,21 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
     } else {
       while (wgs_of(gs) < 256 && narrower(gs, 1) != gs) gs = narrower(gs, 1);
     }
-  } else if (wgs_of(gs) < 2048 && gs * cpg * size % 128 == 0) {
+  } else if ((!grad || wgs_of(gs) < 2048) && gs * cpg * size % 128 == 0) {
     for (int i = least; i < gs; ++i)
       if (fits(i) && i * cpg * size == 64) gs = i;
   }
   // As many threads as leave each a few vectors: six where there are many workgroups, but three in the forward pass while a vector lies
-  // in one group (else the sums over a slab grow with the threads).  LDS for three workgroups of 512 threads on a CU, five
-  // (forward) or four smaller ones (256 boards of 128 bf16 channels, forward: 512 threads 15.5 us, 256 threads 16.0; of float32
-  // 30 / 40 us; the gradient in bf16 with 256 threads: 52 KB 34 us, 40 KB 28 us, with 512 31 us).
+  // in one group (else the sums over a slab grow with the threads).  LDS for three workgroups of 512 threads on a CU in the
+  // forward pass, two in the gradient whose sums need little of it; five or four smaller ones (2,048 boards of 128 bf16
+  // channels, forward: 52 KB 123 us, 40 KB 126; the gradient 62 KB 227 us, 52 KB 235, but 1,000 boards of 120 float32 channels 50
+  // and 45; 256 boards of 128 bf16 channels with 256 threads: 52 KB 34 us, 40 KB 28 us, with 512 threads 31).
   const int64_t of = (positions + chunks - 1) / chunks, wgs = wgs_of(gs) * chunks;
   const int few = wgs < 64 ? 2 : wgs < 512 || (!grad && cpg % widest == 0) ? 3 : 6;
   p.threads = 64;
   while (p.threads < NORM_THREADS && (p.threads < gs * cpg / widest || vectors_at(p.threads, of) > few)) p.threads *= 2;
-  const int most = p.threads == NORM_THREADS ? 52 << 10 : grad ? 40 << 10 : 32 << 10;
+  const bool pow2 = is_pow2(gs * cpg / widest);
+  const int most = p.threads == NORM_THREADS ? (grad && pow2 ? 62 << 10 : 52 << 10) : grad ? 40 << 10 : 32 << 10;
   NormCut& c = p.cut;
   p.vec = vec ? vec : widest;
   c.slab_groups = gs;
@@ -1248,6 +1252,10 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
     c.scratch = p.threads * (cpg % p.vec == 0 ? 1 : p.vec) + 2 * gs;
   }
   c.scratch = (c.scratch + 3) & ~3;
+  if (c.scratch * 4 > 64 << 10) {   // (a group of more than 4,090 channels: as one that is wider than a workgroup's vectors)
+    c.rows = 0;
+    return p;
+  }
   const int64_t vectors = (c.chunk + c.rows - 1) / c.rows, row = (int64_t)p.threads * p.vec * size * (1 + grad + residual);
   const int64_t room = most > c.scratch * 4 ? (most - c.scratch * 4) / row : 0;
   c.staged = (int)(vectors < room ? vectors : room);
@@ -1325,7 +1333,8 @@ int check_norm(const goenv_norm* p, bool grad) {
   if (p->param_dtype != GOENV_DT_F32 && p->param_dtype != p->dtype)
     return fail("goenv_group_norm_act: param_dtype must be GOENV_DT_F32 or dtype");
   if (p->n < 0 || p->positions < 0 || p->channels < 0) return fail("goenv_group_norm_act: a size is negative");
-  if (p->positions > INT32_MAX) return fail("goenv_group_norm_act: more than 2^31 - 1 positions");
+  if (p->positions > INT32_MAX || p->channels > 1 << 24)
+    return fail("goenv_group_norm_act: more than 2^31 - 1 positions or 2^24 channels");
   if (p->groups <= 0 || p->channels % p->groups) return fail("goenv_group_norm_act: groups must divide channels");
   if (p->act < GOENV_ACT_NONE || p->act > GOENV_ACT_SILU) return fail("goenv_group_norm_act: act must be a GOENV_ACT_*");
   if (!(p->eps >= 0.f) || isinf(p->eps)) return fail("goenv_group_norm_act: eps must be finite and not negative");

@@ -63,6 +63,8 @@ NORM = [
     (300, 24, 6, (2, 2), BF16, "leaky_relu", False, F32),
     (2, 5000, 1, (3,), BF16, "leaky_relu", True, F32),          # groups wider than a workgroup's vectors
     (2, 1025, 1, (5,), F32, "silu", False, F32),
+    (2, 4096, 1, (7,), BF16, "silu", True, F32),                # ... or than their sums in LDS
+    (3, 3000, 1, (9,), F16, "relu", False, F32),
     (130, 96, 32, (25, 25), F16, "relu", True, F32),
     (40, 15, 5, (23, 9), BF16, "silu", True, F32),
     (3, 240, 24, (50, 51), BF16, "leaky_relu", True, F32),
