@@ -53,13 +53,13 @@ Tensor main_tensor(py::handle h, const char* name) {
   const Tensor& t = THPVariable_Unpack(h.ptr());
   if (!t.is_cuda() || t.layout() != at::kStrided) refuse(name, " must be a tensor on the GPU");
   if (!is_float_type(t.scalar_type())) refuse(name, " must be float32, bfloat16 or float16 (got ", t.scalar_type(), ")");
-  return t;
+  return t.resolve_neg();   // (the imaginary part of a conjugate: its memory holds the values with the other sign)
 }
 
 Tensor optional_tensor(py::handle h, const char* name) {
   if (h.is_none()) return Tensor();
   if (!THPVariable_Check(h.ptr())) refuse(name, " must be a tensor (got ", py::str(py::type::handle_of(h)).cast<std::string>(), ")");
-  return THPVariable_Unpack(h.ptr());
+  return THPVariable_Unpack(h.ptr()).resolve_neg();
 }
 
 void check_like(const Tensor& t, const char* name, const Tensor& like, std::initializer_list<at::ScalarType> types, at::IntArrayRef shape) {
@@ -230,7 +230,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     variable_list out(5);
     {
       at::NoGradGuard no_grad;
-      Tensor dy = grads[0];
+      Tensor dy = grads[0].resolve_neg();
       Layout l = layout_of(dy);
       if (!l.ok) {
         dy = dense_like(dy).copy_(dy);
@@ -337,7 +337,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     variable_list out(3);
     if (ctx->needs_input_grad(0)) {
       at::NoGradGuard no_grad;
-      Tensor dy = grads[0];
+      Tensor dy = grads[0].resolve_neg();
       const auto stride = ctx->saved_data["stride"].toIntVector();
       if (!same_order(dy, stride)) dy = at::empty_strided(dy.sizes(), stride, dy.options()).copy_(dy);
       out[0] = dropout_run(dy, Tensor(), ctx->saved_data["p"].toDouble(), rng, ctx->saved_data["site"].toInt());
@@ -449,7 +449,7 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
     variable_list out(3);
     {
       at::NoGradGuard no_grad;
-      Tensor dy = grads[0];
+      Tensor dy = grads[0].resolve_neg();
       if (dy.size(1) != 1 && dy.stride(1) != 1) dy = dy.contiguous();
       Needs needs{ctx};
       if (needs(logits)) out[0] = at::empty(logits.sizes(), logits.options());
@@ -523,7 +523,7 @@ Tensor policy_logits(py::handle plogits, py::handle plegal, py::handle pbits, py
       how.scalar[i] = (float)number(given[i], (std::string(names[i]) + " must be a tensor [rows] or it").c_str());
       continue;
     }
-    const Tensor& t = THPVariable_Unpack(given[i].ptr());
+    const Tensor t = optional_tensor(given[i], names[i]);
     check_like(t, names[i], logits, {at::kFloat}, {rows});
     if (!t.is_contiguous()) refuse(names[i], " must be contiguous");
     if (t.requires_grad()) refuse(names[i], " has no gradient (detach it)");

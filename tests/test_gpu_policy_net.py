@@ -247,3 +247,31 @@ def test_the_net_with_group_norm_and_dropout(ops, dtype):
 def test_the_commands_that_use_them(cmd):
     out = subprocess.run([sys.executable, "-u", os.path.join(ROOT, cmd[0])] + cmd[1:], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and ("cfg3 train" in out.stdout or "cfg5" in out.stdout), out.stdout[-2000:] + out.stderr[-2000:]
+
+
+def test_views_that_negate(ops):
+    """A view may say that its memory holds the values with the other sign (the imaginary part of a conjugate): arguments,
+    rules and gradients count with their values."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    randn = lambda *s: torch.randn(*s, device="cuda", generator=g)                       # noqa: E731
+
+    def other(v):
+        v = torch._neg_view(-v)
+        assert v.is_neg()
+        return v
+    assert torch.complex(randn(3), randn(3)).conj().imag.is_neg()
+    rng = torch.tensor([3, 0], device="cuda")
+    x, r = (randn(3, 5, 8).transpose(1, 2) for _ in range(2))
+    w, b, l, t, past = randn(8), randn(8), randn(4, 9), randn(4).abs() + 0.5, torch.randint(0, 9, (4, 3), device="cuda", generator=g)
+
+    def same(run, *args):
+        for got, want in zip(run(*[other(a) for a in args]), run(*args)):
+            assert torch.equal(got, want)
+    same(lambda x, r, w, b: (ops.group_norm_act(x, 2, w, b, act="silu", residual=r),), x, r, w, b)
+    same(lambda x, r, rng: (ops.dropout(x, 0.5, rng, residual=r),), x, r, rng)
+    same(lambda l, b, t, past: (ops.policy_logits(l, bias=b, history=past, temperature=t, presence=t, out="probs"),), l, randn(9), t, past)
+    leaves = [v.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for v in (x, w, l)]
+    same(lambda dy: torch.autograd.grad(ops.group_norm_act(leaves[0], 2, leaves[1], act="silu"), leaves[:2], dy), r)
+    same(lambda dy: torch.autograd.grad(ops.dropout(leaves[0], 0.5, rng), leaves[0], dy), r)
+    same(lambda dy: torch.autograd.grad(ops.policy_logits(leaves[2], out="log_probs"), leaves[2], dy), randn(4, 9))
