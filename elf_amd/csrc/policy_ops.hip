@@ -1367,11 +1367,12 @@ int check_logits(const goenv_logit_rules* p, bool grad) {
   if (p->rows < 0 || p->cols < 0 || p->cols > (1 << 28)) return fail("goenv_policy_logits: rows or cols out of range");
   if (p->legal && p->legal_bits) return fail("goenv_policy_logits: legal or legal_bits, not both");
   if (p->history && (p->history_max < 0 || p->history_max > (1 << 28))) return fail("goenv_policy_logits: history_max out of range");
-  if (!p->row_temperature && !(p->temperature > 0.f && isfinite(p->temperature)))
-    return fail("goenv_policy_logits: temperature must be positive and finite");
+  auto divides = [](float v) { return v > 0.f && isfinite(v) && isfinite(1.f / v); };   // (the kernels multiply by the inverse)
+  if (!p->row_temperature && !divides(p->temperature))
+    return fail("goenv_policy_logits: temperature must be positive and finite, with a finite inverse");
   if (p->history) {
-    if (!p->row_repetition && !(p->repetition > 0.f && isfinite(p->repetition)))
-      return fail("goenv_policy_logits: repetition must be positive and finite");
+    if (!p->row_repetition && !divides(p->repetition))
+      return fail("goenv_policy_logits: repetition must be positive and finite, with a finite inverse");
     if ((!p->row_presence && !isfinite(p->presence)) || (!p->row_frequency && !isfinite(p->frequency)))
       return fail("goenv_policy_logits: presence and frequency must be finite");
   }

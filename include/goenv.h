@@ -544,7 +544,7 @@ int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* r
  *   history     int32, or int64 if history_i64, [rows][history_max]; entries outside [0, cols) (a pass) are
  *               skipped; history_len int32 [rows], clamped to 0 .. history_max, NULL = history_max
  *   repetition, presence, frequency, temperature: float32 [rows], or NULL = the scalar of that name.  A row's
- *               values are used as they are (the scalars must be > 0, finite, finite, > 0).
+ *               values are used as they are (the scalars must be finite, those that divide > 0 with a finite inverse).
  *   stats       float32 [rows][2], the row's largest z and sum exp(z - largest): for the backward pass of
  *               LOG_PROBS and PROBS; else NULL
  *   workspace   at least goenv_policy_logits_workspace(..., 0) bytes, 16-byte aligned (NULL if that is 0)

@@ -158,6 +158,7 @@ def _rules(**change):
     (dict(cols=-1), "range"), (dict(cols=1 << 31), "range"), (dict(legal=256, legal_bits=256), "not both"),
     (dict(bias=256, bias_dtype=2), "bias_dtype"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
     (dict(temperature=float("inf")), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=2.0 ** -129), "temperature"), (dict(history=256, history_max=1, repetition=2.0 ** -129), "repetition"),
     (dict(history=256, history_max=-1), "history_max"), (dict(history=256, history_max=1, repetition=0.0), "repetition"),
     (dict(history=256, history_max=1, repetition=float("inf")), "repetition"),
     (dict(history=256, history_max=1, presence=float("nan")), "presence"),
