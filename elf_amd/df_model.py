@@ -73,8 +73,8 @@ class PolicyValueNet(nn.Module):
 
     def forward(self, x, legal=None, temperature=1.0):
         """x: the batch (anything answering ["s"]) or the planes tensor [B, 25, 19, 19].  legal: the environment's mask [B, 361]:
-        pi is then taken over the legal points, its logits over `temperature` (a row without one gives zeros, for
-        which the environment falls back to its uniform policy)."""
+        pi is then taken over the legal points (a row without one gives zeros, for which the environment falls back to its
+        uniform policy).  temperature: a number, or a float32 tensor [B]; pi's logits are divided by it."""
         s = x if torch.is_tensor(x) else x["s"]
         s = s.to(self.pi_linear.weight.dtype)
         if self.groups:
@@ -84,7 +84,7 @@ class PolicyValueNet(nn.Module):
             s = self._block(i, s)
         d = self.board_size * self.board_size
         logits = self.pi_linear(self._apply_layer(self.pi_final_conv, s).reshape(-1, 2 * d))
-        if legal is None and temperature == 1.0:
+        if legal is None and not torch.is_tensor(temperature) and temperature == 1.0:
             pi = torch.softmax(logits, dim=1)
         else:
             pi = policy_ops.policy_logits(logits, legal=legal, temperature=temperature, out="probs", dtype=torch.float32)

@@ -234,6 +234,8 @@ def test_the_net_with_group_norm_and_dropout(ops, dtype):
         net.next_step()
         assert torch.equal(net(s, legal, 0.8)["pi"], one["pi"])
     assert one["pi"].dtype == torch.float32 and not one["pi"][legal == 0].any()
+    with torch.no_grad():                                                                # a temperature per position
+        assert torch.equal(net(s, temperature=torch.full((5,), 0.8, device="cuda"))["pi"], net(s, temperature=0.8)["pi"])
     sums = one["pi"].double().sum(1).cpu()
     # 361 probabilities of half a step each, the sum they were divided by off by (24 + 64) roundings
     assert float((sums[:4] - 1).abs().max()) <= (361 + 88) * 2.0 ** -24 and float(sums[4]) == 0
