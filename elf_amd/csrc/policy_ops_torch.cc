@@ -3,11 +3,13 @@
 // In C++ because the backward pass of a small tensor costs more in Python (the engine's thread has to take the interpreter's
 // lock) than its kernels take: a 256 x 722 dropout forward and backward 97 us there.  Every kernel is reached through the C-ABI.
 #include <ATen/ATen.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -111,11 +113,28 @@ struct Needs {
   bool operator()(const Tensor& t) { return t.defined() && ctx->needs_input_grad(edge++); }
 };
 
+// A leaf's gradients are accumulated on the stream where its first graph that still lives was made.  If that is the default
+// stream, which no capture can take in, the backward pass of a graph under capture makes it wait for the capture: torch
+// ends the process.  So such a call is refused.
+void check_capture(const Tensor& t) {
+  if (!t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto made = node->stream();
+  const auto now = c10::hip::getCurrentHIPStream(t.device().index()), eager = c10::hip::getDefaultHIPStream(t.device().index());
+  if (made && made->id() == eager.id() && now != eager && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    refuse("a graph made outside the capture still lives and shares a leaf with this call: delete what it returned, or capture with leaves of its own");
+}
+
 bool wants_grad(std::initializer_list<Tensor> all) {
   if (!at::GradMode::is_enabled()) return false;
+  bool wants = false;
   for (const Tensor& t : all)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
+    if (t.defined() && t.requires_grad()) {
+      check_capture(t);
+      wants = true;
+    }
+  return wants;
 }
 
 // ---- group norm -----------------------------------------------------------------------------------

@@ -114,6 +114,39 @@ def test_a_training_step_in_a_captured_graph(ops):
         before = out[1].clone()
 
 
+def test_a_capture_refuses_leaves_of_a_living_eager_graph(ops):
+    """The forward call is refused, before torch's engine would tie the default stream to the capture.  Without gradients, after
+    the eager graph's end, or with a graph made on another stream that is not the default one, it is captured."""
+    from elf_amd.goenv import GoEnvError
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    x, l = torch.randn(2, 9, 8, device="cuda").transpose(1, 2), torch.randn(2, 8, device="cuda")
+    rng = torch.tensor([1, 0], device="cuda")
+    calls = [lambda: ops.group_norm_act(x, 2, w), lambda: ops.policy_logits(l, bias=w), lambda: ops.dropout(w, 0.5, rng)]
+    want = [run() for run in calls]                                                      # three eager graphs of the leaf
+    grads = [torch.autograd.grad(y.sum(), w, retain_graph=True)[0] for y in want]
+    torch.cuda.synchronize()
+    for run in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with torch.no_grad():
+                out = run()                                                              # (so that the graph is not empty)
+            with pytest.raises(GoEnvError, match="outside the capture"):
+                run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+    want = [y.detach() for y in want]
+    for run, y, gw in zip(calls, want, grads):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+            got = torch.autograd.grad(out, w, torch.ones_like(out))[0]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, y) and torch.equal(got, gw)
+        del out, got
+
+
 def test_two_graphs_side_by_side(ops):
     """Long axes and long rows use workspaces; two captured graphs replayed at the same time on two streams have one each."""
     g = torch.Generator(device="cuda")
