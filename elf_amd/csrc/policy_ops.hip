@@ -158,12 +158,15 @@ struct NormPlace {
   int c0, unit, row, part, count;   // first channel of the slab; the vector of the position; the row; the chunk
   bool on;                          // the thread has a row
 };
+// Workgroups go to the eight XCDs in turn; each XCD takes a run of neighbours, so that what lies next to each other in memory (the
+// slabs of a sample share cache lines) meets in one L2.
+__device__ __forceinline__ uint32_t near_block() {
+  const uint32_t xcd = blockIdx.x & 7, share = gridDim.x >> 3, over = gridDim.x & 7;
+  return xcd * share + (xcd < over ? xcd : over) + (blockIdx.x >> 3);
+}
 __device__ __forceinline__ NormPlace norm_place(const goenv_norm& P, const NormCut& cut) {
   NormPlace q;
-  // Workgroups go to the eight XCDs in turn; each XCD takes a run of neighbours, so that what lies next to each other in memory (the
-  // slabs of a sample share cache lines) meets in one L2.
-  const uint32_t xcd = blockIdx.x & 7, share = gridDim.x >> 3, over = gridDim.x & 7;
-  uint32_t b = xcd * share + (xcd < over ? xcd : over) + (blockIdx.x >> 3);
+  uint32_t b = near_block();
   q.part = (int)(b % (uint32_t)cut.chunks);
   b /= (uint32_t)cut.chunks;
   q.c0 = (int)(b % (uint32_t)cut.slabs) * cut.width;
@@ -544,6 +547,198 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
       });
 }
 
+// Few positions (a feature vector a sample, a small board): a slab would leave most of a workgroup idle.  A team of 1 to 64
+// lanes of one wave takes a sample's group instead, NK vectors a lane, all in registers; sums are exchanges within the team,
+// without LDS and barriers (65,536 x 512 bf16 features in 8 groups: 352 -> 26 us, a copy's time; the gradient 910 -> 49 us, 4.1 TB/s).  A workgroup has the teams of slab_groups groups of `slots` samples and takes samples in strides,
+// so that the gradient's channel sums stay in registers until the end.
+struct FewCut {
+  int team, units, rows;         // lanes of a team; its vectors of a position; the positions that it has at a time
+  int slab_groups, slabs, slots;
+  int64_t strides;               // workgroups of a slab
+};
+constexpr int FEW_THREADS = 256;
+
+struct FewPlace {
+  int lane, unit, group, slab;
+  int64_t stride, first;         // the workgroup's number in its slab; the first sample
+  bool on;                       // the team has a group
+};
+__device__ __forceinline__ FewPlace few_place(const goenv_norm& P, const FewCut& cut) {
+  FewPlace q;
+  const uint32_t b = near_block();
+  q.slab = (int)(b % (uint32_t)cut.slabs);
+  q.stride = b / (uint32_t)cut.slabs;
+  const int team = threadIdx.x / cut.team, slot = team / cut.slab_groups;
+  q.lane = threadIdx.x % cut.team;
+  q.unit = q.lane % cut.units;
+  q.group = q.slab * cut.slab_groups + team % cut.slab_groups;
+  q.on = slot < cut.slots && q.group < P.groups;
+  q.first = q.on ? q.stride * cut.slots + slot : P.n;
+  if (!q.on) q.group = 0;
+  return q;
+}
+// The lane's positions; behind the last one, that one again
+template <int NK>
+__device__ __forceinline__ void few_positions(const goenv_norm& P, const FewCut& cut, const FewPlace& q, int (&at)[NK], bool (&in)[NK]) {
+  const int row = q.lane / cut.units, last = (int)P.positions - 1;
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    const int p = row + k * cut.rows;
+    in[k] = row < cut.rows && p <= last;
+    at[k] = p < last ? p : last;
+  }
+}
+__device__ __forceinline__ float team_sum(float v, int team) {
+  for (int d = 1; d < team; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+template <typename T, int VEC, int NK, bool RES>
+__global__ __launch_bounds__(FEW_THREADS) void k_group_norm_few(goenv_norm P, FewCut cut, T* y) {
+  const int cpg = P.channels / P.groups;
+  const FewPlace q = few_place(P, cut);
+  const int c = q.group * cpg + q.unit * VEC;
+  int at[NK];
+  bool in[NK];
+  few_positions<NK>(P, cut, q, at, in);
+  float w[VEC], b[VEC];
+  load_params<VEC>(P.weight, P.param_dtype, c, 1.f, w);
+  load_params<VEC>(P.bias, P.param_dtype, c, 0.f, b);
+  const float inv_m = 1.f / ((float)P.positions * (float)cpg);
+  for (int64_t sample = q.first; sample < P.n; sample += cut.strides * cut.slots) {
+    const T* x = static_cast<const T*>(P.x) + sample * P.x_sample + c;
+    const T* r = RES ? static_cast<const T*>(P.residual) + sample * P.r_sample + c : nullptr;
+    T* o = y + sample * P.positions * P.channels + c;
+    Pack<T, VEC> a[NK], e[RES ? NK : 1];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) a[k] = load_pack<T, VEC>(x + at[k] * P.x_position);
+    if (RES)
+#pragma unroll
+      for (int k = 0; k < NK; ++k) e[k] = load_pack<T, VEC>(r + at[k] * P.r_position);
+    float mean = 0.f, rstd = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += (float)a[k].v[j];
+      mean += in[k] ? s : 0.f;
+    }
+    mean = team_sum(mean, cut.team) * inv_m;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = (float)a[k].v[j] - mean;
+        s += d * d;
+      }
+      rstd += in[k] ? s : 0.f;
+    }
+    rstd = 1.f / sqrtf(team_sum(rstd, cut.team) * inv_m + P.eps);
+    if (P.stats && q.lane == 0) reinterpret_cast<float2*>(P.stats)[sample * P.groups + q.group] = make_float2(mean, rstd);
+    by_act(P.act, [&](auto act) {
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float z = ((float)a[k].v[j] - mean) * (w[j] * rstd) + b[j];
+          if (RES) z += (float)e[k].v[j];
+          out.v[j] = (T)act_of<decltype(act)::value>(P.slope, z);
+        }
+        if (in[k]) *reinterpret_cast<Pack<T, VEC>*>(o + (int64_t)at[k] * P.channels) = out;
+      }
+    });
+  }
+}
+
+// The gradients.  The workspace: [strides][channels] sums of dz and dz xh, for k_group_norm_param_grad.
+template <typename T, int VEC, int NK, bool RES>
+__global__ __launch_bounds__(FEW_THREADS) void k_group_norm_few_grad(goenv_norm P, FewCut cut, const T* dy0, int64_t dy_sample, int64_t dy_position,
+                                                                     T* dx, T* dr) {
+  __shared__ float lds[2][VEC][FEW_THREADS];
+  const int cpg = P.channels / P.groups;
+  const FewPlace q = few_place(P, cut);
+  const int c = q.group * cpg + q.unit * VEC;
+  int at[NK];
+  bool in[NK];
+  few_positions<NK>(P, cut, q, at, in);
+  float w[VEC], b[VEC], sum1[VEC], sum2[VEC];
+  load_params<VEC>(P.weight, P.param_dtype, c, 1.f, w);
+  load_params<VEC>(P.bias, P.param_dtype, c, 0.f, b);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sum1[j] = sum2[j] = 0.f;
+  const float inv_m = 1.f / ((float)P.positions * (float)cpg);
+  for (int64_t sample = q.first; sample < P.n; sample += cut.strides * cut.slots) {
+    const T* x = static_cast<const T*>(P.x) + sample * P.x_sample + c;
+    const T* r = RES ? static_cast<const T*>(P.residual) + sample * P.r_sample + c : nullptr;
+    const T* dy = dy0 + sample * dy_sample + c;
+    Pack<T, VEC> a[NK], g[NK], e[RES ? NK : 1];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) a[k] = load_pack<T, VEC>(x + at[k] * P.x_position);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) g[k] = load_pack<T, VEC>(dy + at[k] * dy_position);
+    if (RES)
+#pragma unroll
+      for (int k = 0; k < NK; ++k) e[k] = load_pack<T, VEC>(r + at[k] * P.r_position);
+    const float2 st = reinterpret_cast<const float2*>(P.stats)[sample * P.groups + q.group];
+    const float mean = st.x, rstd = st.y;
+    float xh[NK][VEC], dz[NK][VEC], m1 = 0.f, m2 = 0.f;
+    by_act(P.act, [&](auto act) {
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float h = ((float)a[k].v[j] - mean) * rstd;
+          float z = h * w[j] + b[j];
+          if (RES) z += (float)e[k].v[j];
+          const float d = act_grad<decltype(act)::value>(P.slope, z, (float)g[k].v[j]);
+          xh[k][j] = h;
+          dz[k][j] = d;
+          sum1[j] += in[k] ? d : 0.f;
+          sum2[j] += in[k] ? d * h : 0.f;
+          m1 += in[k] ? d * w[j] : 0.f;
+          m2 += in[k] ? d * w[j] * h : 0.f;
+        }
+    });
+    m1 = team_sum(m1, cut.team) * inv_m;
+    m2 = team_sum(m2, cut.team) * inv_m;
+    const int64_t o = sample * P.positions * P.channels + c;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      Pack<T, VEC> ox, orr;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        orr.v[j] = (T)dz[k][j];
+        ox.v[j] = (T)(rstd * (dz[k][j] * w[j] - m1 - xh[k][j] * m2));
+      }
+      if (in[k]) {
+        if (dx) *reinterpret_cast<Pack<T, VEC>*>(dx + o + (int64_t)at[k] * P.channels) = ox;
+        if (dr) *reinterpret_cast<Pack<T, VEC>*>(dr + o + (int64_t)at[k] * P.channels) = orr;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    lds[0][j][threadIdx.x] = sum1[j];
+    lds[1][j][threadIdx.x] = sum2[j];
+  }
+  __syncthreads();
+  float2* part = static_cast<float2*>(P.workspace) + q.stride * P.channels;
+  const int left = P.groups - q.slab * cut.slab_groups, width = (left < cut.slab_groups ? left : cut.slab_groups) * cpg;
+  for (int ch = threadIdx.x; ch < width; ch += FEW_THREADS) {
+    const int group = ch / cpg, in_group = ch % cpg, j = in_group % VEC, from = group * cut.team + in_group / VEC;
+    float s1 = 0.f, s2 = 0.f;
+    for (int slot = 0; slot < cut.slots; ++slot)
+      for (int row = 0; row < cut.rows; ++row) {
+        const int t = from + slot * cut.slab_groups * cut.team + row * cut.units;
+        s1 += lds[0][j][t];
+        s2 += lds[1][j][t];
+      }
+    part[q.slab * cut.slab_groups * cpg + ch] = make_float2(s1, s2);
+  }
+}
+
 // dbias and dweight: the sums of the samples' (and chunks') parts, 16 channels (a cache line) a workgroup, 64 rows at a time
 __global__ __launch_bounds__(1024) void k_group_norm_param_grad(const float2* part, int64_t rows, int channels, int param_dtype, void* dweight,
                                                                 void* dbias) {
@@ -560,6 +755,7 @@ __global__ __launch_bounds__(1024) void k_group_norm_param_grad(const float2* pa
   lds[row][col] = make_float2(a, b);
   __syncthreads();
   if (row != 0 || c >= channels) return;
+#pragma unroll 8
   for (int i = 1; i < 64; ++i) {
     a += lds[i][col].x;
     b += lds[i][col].y;
@@ -1263,6 +1459,56 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   return p;
 }
 
+// The cut into teams, or none (team 0).  `vec` 0: the widest vector; else what the arrays' alignment allows.
+struct FewPlan {
+  FewCut cut;
+  int vec, nk;
+};
+FewPlan few_plan(int64_t n, int64_t positions, int channels, int groups, int dtype, bool grad, int vec = 0) {
+  FewPlan p = {};
+  const int cpg = channels / groups, most = dtype == GOENV_DT_F32 ? 4 : 8;
+  p.vec = cpg % most == 0 ? most : dtype != GOENV_DT_F32 && cpg % 2 == 0 ? 2 : 1;
+  if (vec && vec < p.vec) p.vec = vec;
+  FewCut& c = p.cut;
+  c.units = cpg / p.vec;
+  // Vectors of 16 bytes: up to four of a lane in the forward pass, two in the gradient (2,048 boards of 7 x 7 x 128 bf16 channels in 8
+  // groups, slabs against teams: 21 -> 15 us, 41 -> 34 us; 9 x 9, 1,024 of them: 17 -> 14, but 34 -> 43 us).  Narrower ones, whose loads
+  // use a part of a cache line each: a few positions (16,384 samples of 128 bf16 channels in 32 groups, 16 positions: 123 -> 36 us,
+  // 113 -> 91, but 25 of them 69 -> 45, 69 -> 91; of 120 float32 channels in 24 groups, 8 positions: 62 -> 53, 88 -> 86, but 16 of
+  // them 72 -> 101, 123 -> 204).
+  const int vectors = grad ? 2 : 4;
+  if (c.units > 64 || (p.vec < most && positions > (p.vec == 1 ? 8 : 16))) return p;
+  auto of_lane = [&](int team) { return (positions + team / c.units - 1) / (team / c.units); };
+  int team = 1;
+  while (team < c.units) team *= 2;
+  const int want = n * groups <= 1024 ? 1 : vectors;   // (few teams: more lanes each; 64 boards of 5 x 5 4.3 -> 3.6 us)
+  while (team < 64 && of_lane(team) > want) team *= 2;
+  if (of_lane(team) > vectors) return p;
+  c.team = team;
+  c.rows = team / c.units;
+  p.nk = of_lane(team) > 2 ? 4 : (int)of_lane(team);
+  const int teams = FEW_THREADS / team;
+  c.slab_groups = groups < teams ? groups : teams;
+  c.slabs = (groups + c.slab_groups - 1) / c.slab_groups;
+  c.slots = teams / c.slab_groups;
+  c.strides = (n + c.slots - 1) / c.slots;
+  // A workgroup takes several samples where there are many, for its weights (65,536 x 512 bf16 features: 35 -> 25 us) and its channel
+  // sums: the more rows of them, the longer k_group_norm_param_grad reads.
+  auto most_workgroups = [&](int64_t workgroups) {
+    const int64_t strides = (workgroups + c.slabs - 1) / c.slabs;
+    if (c.strides > strides) c.strides = strides;
+  };
+  most_workgroups(!grad ? 4096 : c.strides / 8 * c.slabs > 2048 ? 2048 : c.strides / 8 * c.slabs < 512 ? 512 : c.strides / 8 * c.slabs);
+  return p;
+}
+// f(vectors of a lane)
+template <typename F>
+void by_vectors(int nk, F f) {
+  if (nk == 1) f(Int<1>());
+  else if (nk == 2) f(Int<2>());
+  else f(Int<4>());
+}
+
 // The widest vector that the arrays' alignment allows
 int norm_fit(const goenv_norm* a, const void* dy, int64_t dy_sample, int64_t dy_position, const void* o1, const void* o2) {
   const int size = a->dtype == GOENV_DT_F32 ? 4 : 2, vec = norm_vec(a->channels, a->dtype);
@@ -1396,7 +1642,14 @@ extern "C" {
 int64_t goenv_group_norm_workspace(int64_t n, int64_t positions, int channels, int groups, int dtype, int grad) {
   if (n <= 0 || positions <= 0 || channels <= 0 || groups <= 0 || channels % groups) return 0;
   const NormPlan plan = norm_plan(n, positions, channels, groups, dtype, true, grad);
-  if (grad) return n * plan.cut.chunks * channels * (int64_t)sizeof(float2);
+  if (grad) {
+    int64_t rows = n * plan.cut.chunks;
+    for (int vec : {0, 1, 2}) {
+      const FewPlan few = few_plan(n, positions, channels, groups, dtype, true, vec);
+      if (few.cut.team && few.cut.strides > rows) rows = few.cut.strides;
+    }
+    return rows * channels * (int64_t)sizeof(float2);
+  }
   return plan.split ? n * plan.cut.chunks * groups * (int64_t)sizeof(float2) : 0;
 }
 
@@ -1406,6 +1659,23 @@ int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream) {
   if (!y || !aligned(y, p->dtype)) return fail("goenv_group_norm_act: y is required, aligned to its elements");
   ON_DEVICE(p->device, "goenv_group_norm_act");
   const goenv_norm q = with_act(p);
+  const FewPlan few = few_plan(q.n, q.positions, q.channels, q.groups, q.dtype, false, norm_fit(&q, nullptr, 0, 0, y, nullptr));
+  if (few.cut.team) {
+    by_dtype(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      by_vec<T>(few.vec, [&](auto v) {
+        by_vectors(few.nk, [&](auto k) {
+          constexpr int VEC = decltype(v)::value, NK = decltype(k)::value;
+          auto go = [&](auto f) {
+            hipLaunchKernelGGL(f, dim3((unsigned)(few.cut.strides * few.cut.slabs)), dim3(FEW_THREADS), 0, S(stream), q, few.cut, static_cast<T*>(y));
+          };
+          q.residual ? go(k_group_norm_few<T, VEC, NK, true>) : go(k_group_norm_few<T, VEC, NK, false>);
+        });
+      });
+    });
+    HIPCHK(hipGetLastError());
+    return 0;
+  }
   const NormPlan plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, false, norm_fit(&q, nullptr, 0, 0, y, nullptr));
   if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks) return fail("goenv_group_norm_act: too many samples for one launch");
   by_dtype(p->dtype, [&](auto t) {
@@ -1446,7 +1716,24 @@ int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sa
   ON_DEVICE(p->device, "goenv_group_norm_act_grad");
   const goenv_norm q = with_act(p);
   NormPlan plan = {};
-  if (!empty) {
+  FewPlan few = {};
+  if (!empty) few = few_plan(q.n, q.positions, q.channels, q.groups, q.dtype, true, norm_fit(&q, dy, dy_sample, dy_position, dx, dresidual));
+  if (few.cut.team) {
+    by_dtype(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      by_vec<T>(few.vec, [&](auto v) {
+        by_vectors(few.nk, [&](auto k) {
+          constexpr int VEC = decltype(v)::value, NK = decltype(k)::value;
+          auto go = [&](auto f) {
+            hipLaunchKernelGGL(f, dim3((unsigned)(few.cut.strides * few.cut.slabs)), dim3(FEW_THREADS), 0, S(stream), q, few.cut,
+                               static_cast<const T*>(dy), dy_sample, dy_position, static_cast<T*>(dx), static_cast<T*>(dresidual));
+          };
+          q.residual ? go(k_group_norm_few_grad<T, VEC, NK, true>) : go(k_group_norm_few_grad<T, VEC, NK, false>);
+        });
+      });
+    });
+    HIPCHK(hipGetLastError());
+  } else if (!empty) {
     plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, true, norm_fit(&q, dy, dy_sample, dy_position, dx, dresidual));
     if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks)
       return fail("goenv_group_norm_act_grad: too many samples for one launch");
@@ -1481,7 +1768,7 @@ int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sa
   }
   if (dweight || dbias) {
     hipLaunchKernelGGL(k_group_norm_param_grad, dim3((q.channels + 15) / 16), dim3(1024), 0, S(stream),
-                       static_cast<const float2*>(q.workspace), empty ? 0 : q.n * plan.cut.chunks, q.channels, q.param_dtype, dweight, dbias);
+                       static_cast<const float2*>(q.workspace), empty ? 0 : few.cut.team ? few.cut.strides : q.n * plan.cut.chunks, q.channels, q.param_dtype, dweight, dbias);
     HIPCHK(hipGetLastError());
   }
   return 0;

@@ -69,6 +69,14 @@ NORM = [
     (40, 15, 5, (23, 9), BF16, "silu", True, F32),
     (3, 240, 24, (50, 51), BF16, "leaky_relu", True, F32),
     (2, 128, 128, (40, 41), F32, "none", False, F32),
+    (9000, 512, 1, (), BF16, "relu", True, F32),                # few positions: several samples a workgroup, one after the other
+    (3000, 64, 8, (1,), F32, "silu", False, F32),
+    (700, 120, 24, (2,), BF16, "silu", True, BF16),
+    (33, 6, 6, (3, 3), F16, "relu", False, F32),
+    (500, 960, 320, (2, 2), F32, "leaky_relu", True, F32),      # more groups than a workgroup has teams
+    (70, 80, 2, (3,), BF16, "none", True, None),
+    (40, 264, 1, (3,), F16, "silu", False, F16),
+    (11, 528, 1, (2,), BF16, "leaky_relu", True, F32),          # a wave's lanes do not hold a position
 ]
 ids = lambda v: str(v).replace("torch.", "").replace(" ", "")                             # noqa: E731
 
@@ -132,6 +140,7 @@ def test_group_norm_unaligned(ops):
             def at(n, c, s):
                 return normal(g, n * s * c + k, dtype=dtype)[k:].view(n, s, c).movedim(-1, 1)
             check_norm(ops, at(3, 64, 50), at(3, 64, 50), normal(g, 64 + k)[k:], normal(g, 64 + k)[k:], at(3, 64, 50), 8, "leaky_relu")
+            check_norm(ops, at(7, 64, 3), at(7, 64, 3), None, None, at(7, 64, 3), 8, "silu")
 
 
 def test_group_norm_empty(ops):
@@ -158,7 +167,7 @@ def test_group_norm_non_finite_samples_stay_apart(ops):
             assert torch.equal(part, clean[i, 8 * k:8 * k + 8]) if same[i, k] else bool(torch.isnan(part).all())
 
 
-@pytest.mark.parametrize("case", [NORM[3], NORM[5], NORM[12], NORM[15]], ids=ids)
+@pytest.mark.parametrize("case", [NORM[3], NORM[5], NORM[12], NORM[15], NORM[26], NORM[28]], ids=ids)
 def test_group_norm_gives_equal_bits(ops, case):
     x, r, w, b, dy = norm_inputs(case, 6)
     for t in (x, r, w, b):
