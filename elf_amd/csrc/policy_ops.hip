@@ -71,8 +71,9 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
 // ---- group norm ---------------------------------------------------------------------------------
 //
 // y = act((x - mean) rstd w + b + residual) per sample and group.  Bound by memory: the forward pass has to read x and the residual
-// and write y once (2,048 boards of 128 bf16 channels: 568 MB, 117 us = 4.9 TB/s, what a copy of that size reaches), the
-// backward pass reads x, dy and the residual and writes dx and dresidual (256 boards: 118 MB, 26 us and 3 us for the channels' sums).
+// and write y once (2,048 boards of 128 bf16 channels: 568 MB, 120 us = 4.7 TB/s; a large copy reaches 4.9), the
+// backward pass reads x, dy and the residual and writes dx and dresidual (the same boards: 227 us = 4.2 TB/s; 256 boards, 118 MB: 26 us
+// and 4 us for the channels' sums).
 // So a sample's slab of a few groups is held by one workgroup, in LDS, from the first read to the write: the mean and then the
 // squared deviations about it (not sums of squares, which lose the variance of data far from zero) are taken from LDS.  The loads
 // go to LDS directly, without registers in between: with the slab in registers a thread's loads waited for each other
@@ -871,6 +872,9 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint32_t step, uint32_t 
   return make_uint4(a, b, c, d);
 }
 
+// Bound by memory (11.8 million bf16 elements and a residual: 71 MB, 13 us; without the residual 47 MB, 11 us) as long as the generator
+// stays behind it: 20 products for eight elements of 16 bits each.  32 bits an element would double them, and a stored mask
+// would have to be written and read.  Whole 16-byte vectors a thread, and a block's bits are made while its loads are under way.
 template <typename T>
 struct alignas(16) Eight {
   T v[8];
@@ -920,8 +924,11 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t n, const T* x, const T*
 // A row's columns are cut into slices of threads x NI vectors of VEC columns, one workgroup each, with the slice's columns
 // in registers; how often a column stands in the row's history is counted in LDS (integers: the order does not matter).  Bound by
 // memory for many rows or long ones, by latency for a short one; so a row that fits one slice takes one launch and reads everything
-// once.  Longer rows take a launch for the slices' maxima and sums and one that joins them and computes z again, which costs
-// reading the logits a second time (from the caches) instead of writing and reading z in 32 bits.
+// once (8,192 rows of 361 bf16 columns with a mask and a history: 7.1 us, bound by instructions, some 285 a wave and row, since a row of
+// odd length has no vectors; 64 rows of 131,072 with histories of 2,048, no softmax: 36 MB, 10 us = 3.5 TB/s, bound by the
+// counts in LDS).  Longer rows take a launch for the slices' maxima and sums and one that joins them and computes z again, which costs
+// reading the logits a second time (from the caches) instead of writing and reading z in 32 bits (one row of 131,072:
+// 4.3 and 4.1 us, of which a launch by itself takes 2).
 
 struct LogitCut {
   int threads;             // of a slice

@@ -66,7 +66,8 @@ def dropout(x, p, rng, site=0, residual=None):
 
 
 class DropoutState(nn.Module):
-    """The (seed, step) of a network's dropout layers, as a buffer of it; layers take a site each."""
+    """The (seed, step) of a network's dropout layers, as a buffer of it; layers take a site each.  Data-parallel ranks hold
+    the same buffer: for masks of its own a rank adds rank * sites to its sites."""
 
     def __init__(self, seed=0):
         super().__init__()
