@@ -379,6 +379,10 @@ LOGITS = [
     (3, 70001, F32, "log_probs", None, "none", "row", 0, None),
     (513, 17, F32, "logits", None, "bytes", "shared", 2, torch.int32),
     (9, 2, BF16, "probs", None, "bytes", "none", 0, None),
+    (5, 3307, F32, "log_probs", None, "bits", "shared", 20, torch.int32),      # slices that are no power of two
+    (6, 1537, BF16, "logits", None, "bytes", "row", 30, torch.int64),
+    (3, 20666, F16, "probs", F32, "bits", "shared", 700, torch.int32),
+    (2, 10004, F32, "probs", None, "none", "none", 0, None),
 ]
 
 
