@@ -535,7 +535,7 @@ int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* r
  *   a = (l > 0 ? l / repetition : l * repetition) - presence - frequency * c
  *   z = (a + bias) / temperature              -inf where the row's mask forbids v
  * and out = z (GOENV_OUT_LOGITS), z - log sum exp z (LOG_PROBS) or exp z / sum exp z (PROBS), dense
- * [rows][cols] of type out_dtype (F32, or dtype); computed in float32.  A column whose z is -inf is off,
+ * [rows][cols] of type out_dtype (F32, or dtype); computed in float32 (an exponential below 2^-126 counts as 0).  A column whose z is -inf is off,
  * whatever made it so; a row with every column off gives -inf, or 0 as probabilities (goenv_sample_policy
  * then falls back to its uniform policy).  A forbidden column's logit and bias are not looked at.
  *   legal       u8 [rows][cols], 0 = forbidden (the legal_out of the environment), or NULL

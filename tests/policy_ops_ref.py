@@ -7,6 +7,7 @@ import numpy as np
 import torch
 
 U = 2.0 ** -24
+TINY = 2.0 ** -126               # the smallest normal number
 
 
 def half_step(dtype):
@@ -60,8 +61,9 @@ def group_norm_act(x, groups, weight, bias, eps, act, slope, residual, dy=None):
         z = z + r
         e_z = e_z + 2 * U * (z.abs() + r.abs())
     y, g = act_and_slope(z, act, slope)
-    # silu: |y'| <= 1.1, the exponential and the divisions 8 U and |z| U of the sigmoid; the others: slope at most 1
-    e_y = e_z * 1.1 + (8 + z.abs()) * U * y.abs() if act == "silu" else e_z + 2 * U * y.abs()
+    # silu: |y'| <= 1.1, the exponential and the divisions 8 U and |z| U of the sigmoid, which is 0 where it is below 2^-126 (y = z times
+    # it); the others: slope at most 1
+    e_y = e_z * 1.1 + (8 + z.abs()) * U * y.abs() + TINY * z.abs() if act == "silu" else e_z + 2 * U * y.abs()
     out = dict(y=(y, e_y + half_step(t) * (y.abs() + e_y) + smallest(t)))
     if dy is not None:
         dy = dy.reshape(x.shape)
@@ -173,6 +175,9 @@ def policy_logits(logits, legal=None, bias=None, history=None, history_len=None,
     e_far = e + e.amax(1, keepdim=True) + U * size(z - top) if cols else e               # of z - top
     # an exponential: its argument's error, and a rounding of the argument times log2 e
     e_p = p * (e_far + (e_far * p).sum(1, keepdim=True) + (k + 12) * U + 2 * U * size(z - top) * 2)
+    # the hardware's exponential has no denormals: w < 2^-126 counts as 0, which takes w / total <= w < 2^-126 from its own p, and
+    # from the total less than cols * 2^-126 <= 2^-98 of it (the total is at least 1)
+    e_p = e_p + TINY + 2.0 ** -98 * p
     if out == "logits":
         y, e_y = z, e
     elif out == "probs":

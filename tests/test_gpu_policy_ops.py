@@ -444,6 +444,15 @@ def test_policy_logits_plain_softmax(ops):
             check_logits(ops, (6, cols, F32, out, None, "none"), logits, None, {}, dy)
 
 
+def test_policy_logits_far_tails(ops):
+    """Probabilities down to the smallest that float32 holds, and below."""
+    g = gen(36)
+    logits = -torch.linspace(0, 130, 2000)[torch.randperm(2000, generator=g)].view(4, 500).cuda()
+    for out in ("probs", "log_probs"):
+        case = (4, 500, F32, out, None, "none", "none", 0, None)
+        check_logits(ops, case, logits, None, {}, normal(g, 4, 500))
+
+
 def test_policy_logits_strides_and_types(ops):
     """Rows of any stride and start, masks of truth values, a gradient of another layout or expanded."""
     g = gen(32)
