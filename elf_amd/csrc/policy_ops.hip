@@ -1505,7 +1505,8 @@ FewPlan few_plan(int64_t n, int64_t positions, int channels, int groups, int dty
     const int64_t strides = (workgroups + c.slabs - 1) / c.slabs;
     if (c.strides > strides) c.strides = strides;
   };
-  most_workgroups(!grad ? 4096 : c.strides / 8 * c.slabs > 2048 ? 2048 : c.strides / 8 * c.slabs < 512 ? 512 : c.strides / 8 * c.slabs);
+  const int64_t eight_samples = c.strides / 8 * c.slabs;   // workgroups that take eight each
+  most_workgroups(!grad ? 4096 : eight_samples > 2048 ? 2048 : eight_samples < 512 ? 512 : eight_samples);
   return p;
 }
 // f(vectors of a lane)
