@@ -1398,7 +1398,8 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   };
   // Fewer workgroups than CUs: slabs get narrower, to half lines at first.  If that leaves them too few or too long, the axis is cut
   // into chunks of eight vectors a thread instead (64 x 100 x 100 positions of 64 bf16 channels: 134 -> 66 us, 250 -> 139 us;
-  // two images of 128 x 128 x 256 56 -> 16, 81 -> 26 us).  Half lines are as good while the slab is staged whole,
+  // two images of 128 x 128 x 256 56 -> 16, 81 -> 26 us; 20 x 45 x 45 x 64, 16 vectors uncut and cut: 9 and 13, 17 and 23 us), or as few as
+  // give each CU a workgroup, but three (64 x 64 x 512 with eight and three: 12.1 and 9.5 us, 21 and 16 us).  Half lines are as good while the slab is staged whole,
   // and keep the last round of workgroups short: the forward pass takes them, the gradient while it has few workgroups (512 boards
   // of 256 bf16 channels, forward: 70 us with lines, 67 with half lines; 2,048 boards of 128, the gradient: 227 and 238; 256
   // boards of 128 float32 channels, the gradient: 62 and 57).
@@ -1412,10 +1413,10 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   if (wgs_of(gs) < 256) {
     const int wide = gs;
     while (wgs_of(gs) < 256 && narrower(gs, 64) != gs) gs = narrower(gs, 64);
-    const int64_t v = vectors_at(NORM_THREADS, positions);
-    if (v > (wgs_of(gs) < 256 ? 12 : 16)) {
+    if (vectors_at(NORM_THREADS, positions) > 16) {
       gs = wide;
-      chunks = (vectors_at(NORM_THREADS, positions) + 7) / 8;
+      const int64_t v = vectors_at(NORM_THREADS, positions), fair = (v * wgs_of(gs) + 255) / 256, each = fair < 3 ? 3 : fair > 8 ? 8 : fair;
+      chunks = (v + each - 1) / each;
       const int64_t most = (2047 + wgs_of(gs)) / wgs_of(gs);
       if (chunks > most) chunks = most;
     } else {
