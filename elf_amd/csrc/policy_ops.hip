@@ -281,10 +281,10 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm(goenv_norm P, NormC
   float w[VEC], b[VEC];
   load_params<VEC>(P.weight, P.param_dtype, c, 1.f, w);
   load_params<VEC>(P.bias, P.param_dtype, c, 0.f, b);
-  staged_here();
 
   float mean[NV], rstd[NV];
   if (PHASE != NORM_APPLY) {
+    staged_here();
     const float inv_m = 1.f / ((float)q.chunk_size * (float)cpg);
 #pragma unroll
     for (int j = 0; j < NV; ++j) mean[j] = rstd[j] = 0.f;
@@ -319,27 +319,41 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm(goenv_norm P, NormC
     }
     if (PHASE == NORM_SUMS) return;
   } else {
-    // mean = sum n_k mean_k / n; the deviations about it: sum of M2_k + n_k (mean_k - mean)^2
+    // mean = sum n_k mean_k / n; the deviations about it: sum of M2_k + n_k (mean_k - mean)^2.  A wave takes every eighth group or so,
+    // four at a time, with their loads under way together (and with the loads to LDS).
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    for (int g = wave; g < cut.slab_groups; g += waves) {
-      const int64_t at = q.sample * P.groups + q.c0 / cpg + g;
-      const float2* part = static_cast<const float2*>(P.workspace) + at * cut.chunks;
-      const float inv_m = 1.f / ((float)P.positions * (float)cpg);
-      auto size = [&](int k) { return (float)((k + 1) * cut.chunk < P.positions ? cut.chunk : P.positions - k * cut.chunk) * (float)cpg; };
-      float m = 0.f, s = 0.f;
-      for (int k = lane; k < cut.chunks; k += 64) m += size(k) * part[k].x;
-      m = wave_sum(m);
-      m *= inv_m;
-      for (int k = lane; k < cut.chunks; k += 64) {
-        const float2 v = part[k];
-        s += v.y + size(k) * (v.x - m) * (v.x - m);
+    const float inv_m = 1.f / ((float)P.positions * (float)cpg);
+    const float2* parts = static_cast<const float2*>(P.workspace) + (q.sample * P.groups + q.c0 / cpg) * cut.chunks;
+    auto size = [&](int k) { return (float)((k + 1) * cut.chunk < P.positions ? cut.chunk : P.positions - k * cut.chunk) * (float)cpg; };
+    const float size0 = lane < cut.chunks ? size(lane) : 0.f;
+    for (int g0 = wave; g0 < cut.slab_groups; g0 += 4 * waves) {
+      float2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int g = g0 + i * waves;
+        v[i] = parts[(int64_t)(g < cut.slab_groups ? g : g0) * cut.chunks + (lane < cut.chunks ? lane : 0)];
       }
-      s = wave_sum(s);
-      s = 1.f / sqrtf(s * inv_m + P.eps);
-      if (lane == 0) {
-        lds[2 * g] = m;
-        lds[2 * g + 1] = s;
-        if (P.stats && q.part == 0) reinterpret_cast<float2*>(P.stats)[at] = make_float2(m, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int g = g0 + i * waves;
+        if (g >= cut.slab_groups) break;
+        const float2* part = parts + (int64_t)g * cut.chunks;
+        float m = size0 * v[i].x, s = lane < cut.chunks ? v[i].y : 0.f;
+        for (int k = lane + 64; k < cut.chunks; k += 64) m += size(k) * part[k].x;
+        m = wave_sum(m);
+        m *= inv_m;
+        s += size0 * (v[i].x - m) * (v[i].x - m);
+        for (int k = lane + 64; k < cut.chunks; k += 64) {
+          const float2 u = part[k];
+          s += u.y + size(k) * (u.x - m) * (u.x - m);
+        }
+        s = wave_sum(s);
+        s = 1.f / sqrtf(s * inv_m + P.eps);
+        if (lane == 0) {
+          lds[2 * g] = m;
+          lds[2 * g + 1] = s;
+          if (P.stats && q.part == 0) reinterpret_cast<float2*>(P.stats)[q.sample * P.groups + q.c0 / cpg + g] = make_float2(m, s);
+        }
       }
     }
     __syncthreads();
@@ -349,6 +363,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm(goenv_norm P, NormC
       mean[j] = lds[2 * g];
       rstd[j] = lds[2 * g + 1];
     }
+    staged_here();
   }
 #pragma unroll
   for (int j = 0; j < VEC; ++j) w[j] *= rstd[ONE ? 0 : j];
@@ -403,7 +418,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
     mean[j] = st.x;
     rstd[j] = st.y;
   }
-  staged_here();
+  if (PHASE != NORM_APPLY) staged_here();
   // f(j, xh, dz) for every element of the thread's
   auto each = [&](auto f, auto done) {
     by_act(P.act, [&](auto act) {
@@ -535,6 +550,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_group_norm_grad(goenv_norm P, 
     m1[j] = group[2 * g];
     m2[j] = group[2 * g + 1];
   }
+  if (PHASE == NORM_APPLY) staged_here();
   const int64_t o = (q.sample * P.positions + q.first) * P.channels + c;
   Pack<T, VEC> ox, orr;
   each(
