@@ -1452,7 +1452,10 @@ NormPlan norm_plan(int64_t n, int64_t positions, int channels, int groups, int d
   p.threads = 64;
   while (p.threads < NORM_THREADS && (p.threads < gs * cpg / widest || vectors_at(p.threads, of) > few)) p.threads *= 2;
   const bool pow2 = is_pow2(gs * cpg / widest);
-  const int most = p.threads == NORM_THREADS ? (grad && pow2 ? 62 << 10 : 52 << 10) : grad ? 40 << 10 : 32 << 10;
+  const int shared = p.threads == NORM_THREADS ? (grad && pow2 ? 62 << 10 : 52 << 10) : grad ? 40 << 10 : 32 << 10;
+  // A CU that has one or two workgroups at most gives them all it has (30 images of 42 x 43 x 128 bf16, 240 workgroups: 52 KB 16 us, 152 KB
+  // 14 us, the gradient 27 and 23)
+  const int most = wgs <= 256 ? 152 << 10 : wgs <= 512 ? 76 << 10 : shared;
   NormCut& c = p.cut;
   p.vec = vec ? vec : widest;
   c.slab_groups = gs;
