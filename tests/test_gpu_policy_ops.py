@@ -383,6 +383,9 @@ LOGITS = [
     (6, 1537, BF16, "logits", None, "bytes", "row", 30, torch.int64),
     (3, 20666, F16, "probs", F32, "bits", "shared", 700, torch.int32),
     (2, 10004, F32, "probs", None, "none", "none", 0, None),
+    (5, 9001, BF16, "log_probs", None, "bytes", "row", 300, torch.int32),
+    (2, 12287, F32, "probs", None, "bits", "none", 40, torch.int64),
+    (3, 12289, F16, "probs", F32, "bits", "none", 9, torch.int32),
 ]
 
 
