@@ -496,6 +496,59 @@ __global__ __launch_bounds__(1024) void k_column_sum(const float* part, int64_t 
   store_any(out, dtype, v, a);
 }
 
+__device__ __forceinline__ int64_t row_of(int64_t i, uint32_t width) {   // (64-bit divisions take ten times as long)
+  return i >> 32 ? i / width : (uint32_t)i / width;
+}
+
+// Dense copies of the rules that a gradient reads again: the mask as bits, the histories and their lengths.  Bound by the launch for a batch
+// of boards, by memory for long rows (768 x 361 bytes and four moves a row 2.9 us, 8,192 x 361 and eight moves 3.5, 64 x 131,072 and 2,048 moves
+// 4.2).  A thread makes a word of 32 bytes, loaded by 16 from wherever they start (a wave that makes two words of 64 bytes took 7.3 us for
+// the second case).
+__global__ __launch_bounds__(256) void k_keep_rules(goenv_logit_rules P, int64_t mask_rows, int64_t past_rows, uint32_t* bits, void* history,
+                                                    int32_t* history_len) {
+  const int64_t thread = (int64_t)blockIdx.x * 256 + threadIdx.x, threads = (int64_t)gridDim.x * 256;
+  const uint32_t words = (uint32_t)(P.cols + 31) / 32;
+  if (bits && P.legal) {
+    for (int64_t i = thread; i < mask_rows * words; i += threads) {
+      const int64_t row = row_of(i, words);
+      const uint32_t w = (uint32_t)(i - row * words), cols = (uint32_t)P.cols - w * 32;
+      const uint32_t before = cols < 32 && w ? 32 - cols : 0;   // the last word takes the row's last 32 bytes
+      const uint8_t* from = P.legal + row * P.legal_row + w * 32 - before;
+      uint32_t b[8] = {}, word = 0;
+      if (P.cols >= 32) {
+        __builtin_memcpy(b, from, 32);
+      } else {
+        for (uint32_t k = 0; k < cols; ++k) word |= (uint32_t)(from[k] != 0) << k;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t v = b[k] | (b[k] >> 4 & 0x0f0f0f0fu);   // a byte's lowest bit: whether any of its bits is set
+        v |= v >> 2 & 0x03030303u;
+        v = (v | v >> 1) & 0x01010101u;
+        word |= ((v | v >> 7 | v >> 14 | v >> 21) & 15u) << (4 * k);
+      }
+      bits[i] = word >> before;
+    }
+  } else if (bits) {
+    for (int64_t i = thread; i < mask_rows * words; i += threads) {
+      const int64_t row = row_of(i, words);
+      bits[i] = P.legal_bits[row * P.bits_row + (i - row * words)];
+    }
+  }
+  if (history) {
+    auto copy = [&](auto* from, auto* to) {
+      for (int64_t i = thread; i < past_rows * P.history_max; i += threads) {
+        const int64_t row = row_of(i, (uint32_t)P.history_max);
+        to[i] = from[row * P.history_row + (i - row * P.history_max)];
+      }
+    };
+    if (P.history_i64) copy(static_cast<const int64_t*>(P.history), static_cast<int64_t*>(history));
+    else copy(static_cast<const int32_t*>(P.history), static_cast<int32_t*>(history));
+  }
+  if (history_len)
+    for (int64_t i = thread; i < P.rows; i += threads) history_len[i] = P.history_len[i];
+}
+
 // ---- host: policy logits --------------------------------------------------------------------------
 
 struct LogitPlan {
@@ -711,6 +764,30 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
                        p->bias_dtype, dbias);
     HIPCHK(hipGetLastError());
   }
+  return 0;
+}
+
+int goenv_policy_logits_keep(const goenv_logit_rules* p, uint32_t* legal_bits, void* history, int32_t* history_len, void* stream) {
+  if (!p) return fail("goenv_policy_logits_keep: p is NULL");
+  if (p->rows < 0 || p->cols < 0 || p->cols > (1 << 28)) return fail("goenv_policy_logits_keep: rows or cols out of range");
+  if (p->legal && p->legal_bits) return fail("goenv_policy_logits_keep: legal or legal_bits, not both");
+  if (p->history && (p->history_max < 0 || p->history_max > (1 << 28))) return fail("goenv_policy_logits_keep: history_max out of range");
+  if ((legal_bits && !p->legal && !p->legal_bits) || (history && !p->history) || (history_len && !p->history_len))
+    return fail("goenv_policy_logits_keep: a copy of an array that p does not have");
+  const uintptr_t entry = p->history_i64 ? 7 : 3;
+  if ((((uintptr_t)legal_bits | (uintptr_t)p->legal_bits | (uintptr_t)history_len | (uintptr_t)p->history_len) & 3) ||
+      (((uintptr_t)history | (uintptr_t)p->history) & entry))
+    return fail("goenv_policy_logits_keep: an array is not aligned to its elements");
+  const int64_t mask_rows = legal_bits ? ((p->legal ? p->legal_row : p->bits_row) == 0 && p->rows > 0 ? 1 : p->rows) : 0;
+  const int64_t past_rows = history ? (p->history_row == 0 && p->rows > 0 ? 1 : p->rows) : 0;
+  const int64_t mask = mask_rows * ((p->cols + 31) / 32);
+  const int64_t past = past_rows * p->history_max, lens = history_len ? p->rows : 0;
+  const int64_t most = mask > past ? mask : past, threads = most > lens ? most : lens;
+  if (threads == 0) return 0;
+  ON_DEVICE(p->device, "goenv_policy_logits_keep");
+  hipLaunchKernelGGL(k_keep_rules, dim3(grid_of((threads + 255) / 256, 1 << 14)), dim3(256), 0, S(stream), *p, mask_rows, past_rows, legal_bits,
+                     history, history_len);
+  HIPCHK(hipGetLastError());
   return 0;
 }
 

@@ -446,13 +446,54 @@ Tensor logits_forward(const Tensor& logits, const Tensor& bias, const LogitHow& 
   return out;
 }
 
+// Copies of the mask (as bits), the histories and their lengths, one after the other in a tensor of bytes: the environment writes the next
+// position's into such buffers through plain pointers, of which a saved tensor's version count knows nothing.
+struct Kept {
+  int64_t mask_rows = 0, past_rows = 0, moves = 0, move_bytes = 0, lens = 0;
+  int64_t past_bytes() const { return past_rows * moves * move_bytes; }
+  int64_t bytes(int64_t words) const { return past_bytes() + (mask_rows * words + lens) * (int64_t)sizeof(int32_t); }
+  static Kept of(const goenv_logit_rules& p) {   // (rows that are all the same one are kept once)
+    Kept k;
+    if (p.rows == 0 || p.cols == 0) return k;
+    if (p.legal || p.legal_bits) k.mask_rows = (p.legal ? p.legal_row : p.bits_row) == 0 ? 1 : p.rows;
+    if (!p.history) return k;
+    k.past_rows = p.history_row == 0 ? 1 : p.rows;
+    k.moves = p.history_max;
+    k.move_bytes = p.history_i64 ? sizeof(int64_t) : sizeof(int32_t);
+    if (p.history_len) k.lens = p.rows;
+    return k;
+  }
+  // p with the copies that lie at `base`
+  void to(goenv_logit_rules& p, char* base) const {
+    const int64_t words = (p.cols + 31) / 32;
+    p.history = past_rows ? base : nullptr;
+    p.history_row = past_rows == 1 ? 0 : moves;
+    p.history_max = (int32_t)moves;
+    p.history_i64 = move_bytes == sizeof(int64_t);
+    base += past_bytes();
+    p.legal = nullptr;
+    p.legal_bits = mask_rows ? reinterpret_cast<uint32_t*>(base) : nullptr;
+    p.bits_row = mask_rows == 1 ? 0 : words;
+    base += mask_rows * words * sizeof(uint32_t);
+    p.history_len = lens ? reinterpret_cast<int32_t*>(base) : nullptr;
+  }
+};
+
 struct LogitNode : torch::autograd::Function<LogitNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Maybe& b, const LogitHow& how) {
     const Tensor bias = tensor_of(b);
     const Tensor stats = how.out_kind == GOENV_OUT_LOGITS ? Tensor() : at::empty({logits.size(0), 2}, logits.options().dtype(at::kFloat));
-    Tensor out = logits_forward(logits, bias, how, stats);
-    ctx->save_for_backward({logits, bias, stats, how.legal, how.legal_bits, how.history, how.history_len, how.row[0], how.row[1], how.row[2],
-                            how.row[3]});
+    Tensor out = logits_forward(logits, bias, how, stats), copy;
+    goenv_logit_rules p = logit_args(logits, Tensor(), how, Tensor()), own = p;
+    const Kept kept = Kept::of(p);
+    if (const int64_t bytes = kept.bytes((p.cols + 31) / 32)) {
+      copy = workspace_of(bytes, logits);
+      kept.to(own, static_cast<char*>(copy.data_ptr()));
+      check_rc(goenv_policy_logits_keep(&p, const_cast<uint32_t*>(own.legal_bits), const_cast<void*>(own.history), const_cast<int32_t*>(own.history_len),
+                                        stream_of(logits)));
+    }
+    ctx->save_for_backward({logits, bias, stats, copy, how.row[0], how.row[1], how.row[2], how.row[3]});
+    ctx->saved_data["kept"] = std::vector<int64_t>{kept.mask_rows, kept.past_rows, kept.moves, kept.move_bytes, kept.lens};
     ctx->saved_data["scalar"] = std::vector<double>(how.scalar, how.scalar + 4);
     ctx->saved_data["kind"] = (int64_t)how.out_kind;
     ctx->saved_data["type"] = (int64_t)how.out_type;
@@ -460,8 +501,8 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &bias = saved[1];
-    LogitHow how{saved[3], saved[4], saved[5], saved[6], {saved[7], saved[8], saved[9], saved[10]}, {}, (int)ctx->saved_data["kind"].toInt(),
+    const Tensor &logits = saved[0], &bias = saved[1], &copy = saved[3];
+    LogitHow how{{}, {}, {}, {}, {saved[4], saved[5], saved[6], saved[7]}, {}, (int)ctx->saved_data["kind"].toInt(),
                  (at::ScalarType)ctx->saved_data["type"].toInt()};
     const auto scalar = ctx->saved_data["scalar"].toDoubleVector();
     for (int i = 0; i < 4; ++i) how.scalar[i] = (float)scalar[i];
@@ -474,6 +515,8 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
       if (needs(logits)) out[0] = at::empty(logits.sizes(), logits.options());
       if (needs(bias)) out[1] = at::empty(bias.sizes(), bias.options());
       goenv_logit_rules p = logit_args(logits, bias, how, saved[2]);
+      const auto kept = ctx->saved_data["kept"].toIntVector();
+      if (copy.defined()) Kept{kept[0], kept[1], kept[2], kept[3], kept[4]}.to(p, static_cast<char*>(copy.data_ptr()));
       const int64_t need = goenv_policy_logits_workspace(p.rows, p.cols, p.out_kind, bias.defined() && p.bias_row == 0, 1);
       const Tensor ws = workspace_of(need, logits);
       if (need > 0) p.workspace = ws.data_ptr(), p.workspace_bytes = need;

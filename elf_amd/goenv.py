@@ -126,6 +126,7 @@ _SIGS = {
     "goenv_policy_logits_workspace": (C.c_int64, [C.c_int64, C.c_int64] + [C.c_int] * 3),
     "goenv_policy_logits": (C.c_int, [C.POINTER(LogitRules), C.c_void_p, C.c_void_p]),
     "goenv_policy_logits_grad": (C.c_int, [C.POINTER(LogitRules), C.c_void_p, C.c_int64] + [C.c_void_p] * 3),
+    "goenv_policy_logits_keep": (C.c_int, [C.POINTER(LogitRules)] + [C.c_void_p] * 4),
     "goenv_aug_action": (C.c_int, [C.c_int, C.c_int]),
     "goenv_aug_action_inv": (C.c_int, [C.c_int, C.c_int]),
 }

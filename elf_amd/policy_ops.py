@@ -94,6 +94,7 @@ def policy_logits(logits, legal=None, legal_bits=None, bias=None, history=None, 
     a pass, are skipped; history_len: int32 [rows], how many of a row's entries count (None: all).  repetition,
     presence, frequency, temperature: numbers, or float32 tensors [rows].  dtype: of the result, float32 or the logits'
     type (None: the logits' type).  Forbidden columns give -inf, or 0 as probabilities; so does a row with nothing left.
-    Gradients for logits and bias."""
+    Gradients for logits and bias: of the masks and histories that the call read (it copies them where gradients are wanted,
+    so the environment may write the next position's into the same tensors before the backward pass)."""
     return _ops().policy_logits(logits, legal, legal_bits, bias, history, history_len, repetition, presence, frequency,
                                 temperature, out, dtype)

@@ -551,7 +551,10 @@ int goenv_dropout(int device, int dtype, int64_t n, const void* x, const void* r
  * goenv_policy_logits_grad: dlogits (dense, of type dtype) and dbias (of type bias_dtype; [cols] if bias_row
  * is 0, else dense [rows][cols]) for d_out of type out_dtype, row stride dy_row; either may be NULL.
  * Columns that are off have no gradient and pass none on: what d_out holds there is not looked at.  The
- * penalties and the temperature have none. */
+ * penalties and the temperature have none.  The gradient computes z again: every array of p has to hold what the forward pass read.
+ * goenv_policy_logits_keep copies the arrays that the environment may write the next position's into meanwhile: the mask, as
+ * bits, to legal_bits [rows][(cols + 31) / 32], the histories to history [rows][history_max] (of p's type) and their lengths to
+ * history_len [rows], all dense; each may be NULL.  An array of p whose row stride is 0 gives one row. */
 #define GOENV_OUT_LOGITS 0
 #define GOENV_OUT_LOG_PROBS 1
 #define GOENV_OUT_PROBS 2
@@ -585,6 +588,7 @@ int64_t goenv_policy_logits_workspace(int64_t rows, int64_t cols, int out_kind, 
 int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream);
 int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int64_t dy_row, void* dlogits, void* dbias,
                              void* stream);
+int goenv_policy_logits_keep(const goenv_logit_rules* p, uint32_t* legal_bits, void* history, int32_t* history_len, void* stream);
 
 /* Statistics ---------------------------------------------------------------
  * goenv_finish: score every finished board that has not been counted yet and

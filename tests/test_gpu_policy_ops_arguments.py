@@ -1,0 +1,110 @@
+"""GPU: what the policy-network operators (elf_amd/policy_ops.py) do with arguments that change under them, that carry more
+than values, or that are larger than a launch."""
+import pytest
+import torch
+
+import policy_ops_ref as ref
+from policy_ops_ref import assert_within
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from elf_amd import goenv, policy_ops
+    goenv.load_library()
+    assert torch.cuda.is_available()
+    return policy_ops
+
+
+@pytest.fixture(scope="module")
+def error():
+    from elf_amd import goenv
+    return goenv.GoEnvError
+
+
+def randn(seed, *shape, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def packed(legal):
+    rows, cols = legal.shape
+    bits = torch.zeros(rows, (cols + 31) // 32 * 32, dtype=torch.int64, device=legal.device)
+    bits[:, :cols] = legal != 0
+    w = (bits.view(rows, -1, 32) << torch.arange(32, device=legal.device)).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
+
+
+@pytest.mark.parametrize("mask", ["bytes", "bits", "one row", "none"])
+@pytest.mark.parametrize("out", ["logits", "log_probs", "probs"])
+@pytest.mark.parametrize("moves", [torch.int32, torch.int64], ids=["int32", "int64"])
+def test_the_gradient_goes_by_the_rules_of_its_forward_pass(ops, mask, out, moves):
+    """The environment writes the next position's mask, and moves, into the buffers that the forward pass has read, past torch's
+    count of a tensor's versions: the gradient is that of the old ones, bit for bit."""
+    from elf_amd import goenv
+    boards = 24
+    env = goenv.GoEnv(boards, seed=9, max_ply=722)
+    env.ply_repeat(90, goenv.F_RANDOM_POLICY)
+    legal = env.new(torch.uint8, 361)
+    env.features(legal_out=legal)
+    g = torch.Generator().manual_seed(4)
+    past, other = (torch.randint(-1, 361, (boards, 7), generator=g).to(moves).cuda() for _ in range(2))
+    many, other_many = (torch.randint(0, 8, (boards,), generator=g).to(torch.int32).cuda() for _ in range(2))
+    before = past.clone(), many.clone()
+    bits = packed(legal)
+    given = {"bytes": dict(legal=legal), "bits": dict(legal_bits=bits), "one row": dict(legal=legal[3:4].expand(boards, 361)), "none": {}}[mask]
+    kw = dict(history=past, history_len=many, repetition=1.5, presence=0.5, frequency=0.25, temperature=0.7, out=out)
+    logits, bias, dy = randn(1, boards, 361), randn(2, 361), randn(3, boards, 361)
+    x, b = logits.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    want = torch.autograd.grad(ops.policy_logits(x, bias=b, **given, **kw), (x, b), dy)
+    y = ops.policy_logits(x, bias=b, **given, **kw)
+    old = legal.clone()
+    env.ply_repeat(61, goenv.F_RANDOM_POLICY, legal_out=legal)
+    env.copy_rows(packed(legal), bits)
+    env.copy_rows(other, past)
+    env.copy_rows(other_many[:, None], many[:, None])
+    got = torch.autograd.grad(y, (x, b), dy)
+    assert bool((legal != old).any(1).all()) and torch.equal(past, other) and torch.equal(many, other_many) and torch.equal(bits, packed(legal))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    then = None if mask == "none" else old[3:4].expand(boards, 361) if mask == "one row" else old
+    exact = ref.policy_logits(logits, then, bias, *before, 1.5, 0.5, 0.25, 0.7, out, None, dy)
+    for k, d in zip(("dlogits", "dbias"), got):
+        assert_within(d, exact[k], k)
+    env.close()
+
+
+@pytest.mark.parametrize("rows,cols,start,stride,moves", [
+    (1, 1, 0, 1, 1), (3, 4, 0, 4, 2), (5, 31, 1, 40, 3), (7, 32, 4, 36, 0), (2, 33, 0, 33, 9), (6, 64, 0, 64, 1), (4, 100, 8, 120, 5), (9, 361, 0, 361, 8),
+    (1000, 361, 3, 400, 4), (3, 364, 0, 364, 70), (2, 4101, 0, 4101, 1), (2, 40004, 4, 40012, 700), (70000, 8, 0, 8, 1), (5, 128, 0, 0, 3)])
+def test_copies_of_rules(ops, rows, cols, start, stride, moves):
+    """goenv_policy_logits_keep itself: rows of any start and stride (0: one row), masks of any truth values, and nothing written
+    behind a copy."""
+    import ctypes as C
+    from elf_amd import goenv
+    lib, g = goenv.load_library(), torch.Generator().manual_seed(cols)
+    flat = torch.randint(0, 256, (start + max(rows - 1, 0) * stride + cols,), generator=g).to(torch.uint8)
+    flat = torch.where(torch.rand(flat.shape, generator=g) < 0.5, flat, 0).to(torch.uint8).cuda()
+    legal = flat.as_strided((rows, cols), (stride, 1), start)
+    past = torch.randint(-1, cols, (rows if stride else 1, moves + 3), generator=g).cuda()[:, 1:1 + moves].expand(rows, moves)
+    many = torch.randint(-1, moves + 2, (rows,), generator=g).to(torch.int32).cuda()
+    own, words = rows if stride else 1, (cols + 31) // 32
+    bits_of = packed(legal)
+    for mask in ("legal", "legal_bits"):
+        for wide in (True, False):
+            h = past if wide else past.to(torch.int32) if stride else past[:1].to(torch.int32).expand(rows, moves)
+            p = goenv.LogitRules(device=0, rows=rows, cols=cols, history=h.data_ptr(), history_row=h.stride(0) if moves else 0, history_max=moves,
+                                 history_i64=wide, history_len=many.data_ptr())
+            if mask == "legal":
+                p.legal, p.legal_row = legal.data_ptr(), stride
+            else:
+                p.legal_bits, p.bits_row = bits_of.data_ptr(), words if stride else 0
+            bits = torch.full((own * words + 8,), 77, dtype=torch.int32, device="cuda")
+            moved = torch.full((own * moves + 8,), 78, dtype=h.dtype, device="cuda")
+            lens = torch.full((rows + 8,), 79, dtype=torch.int32, device="cuda")
+            stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            assert lib.goenv_policy_logits_keep(C.byref(p), bits.data_ptr(), moved.data_ptr() if moves else None, lens.data_ptr(), stream) == 0
+            assert torch.equal(bits[:own * words].view(own, words), bits_of[:own]) and bool((bits[own * words:] == 77).all())
+            assert torch.equal(moved[:own * moves].view(own, moves), h[:own]) and bool((moved[own * moves:] == 78).all())
+            assert torch.equal(lens[:rows], many) and bool((lens[rows:] == 79).all())

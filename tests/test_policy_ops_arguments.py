@@ -1,0 +1,37 @@
+"""CPU: what the policy-network operators refuse before they reach a device (elf_amd/policy_ops.py, include/goenv.h)."""
+import ctypes as C
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from elf_amd import goenv
+    return goenv.load_library()
+
+
+def rules(**change):
+    from elf_amd import goenv
+    p = goenv.LogitRules(device=0, dtype=1, out_dtype=0, out_kind=2, rows=2, cols=361, logits=256, logits_row=361, repetition=1.0,
+                         temperature=1.0, stats=256, legal_row=361, bits_row=12, history_row=4)
+    for k, v in change.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("change,args,match", [
+    (dict(rows=-1), (256, None, None), "range"), (dict(cols=(1 << 28) + 1), (256, None, None), "range"),
+    (dict(legal=256, legal_bits=256), (256, None, None), "not both"), (dict(history=256, history_max=-1), (None, 256, None), "history_max"),
+    (dict(), (256, None, None), "does not have"), (dict(legal=256), (None, 256, None), "does not have"),
+    (dict(history=256, history_max=2), (None, 256, 256), "does not have"), (dict(legal=256), (258, None, None), "aligned"),
+    (dict(history=256, history_max=2, history_i64=1), (None, 260, None), "aligned"),
+    (dict(history=260, history_max=2, history_i64=1), (None, 256, None), "aligned"), (dict(legal_bits=257), (256, None, None), "aligned")])
+def test_refused_copies_of_rules(lib, change, args, match):
+    assert lib.goenv_policy_logits_keep(C.byref(rules(**change)), *args, None) == -1 and match in lib.goenv_last_error().decode()
+    assert lib.goenv_policy_logits_keep(None, *args, None) == -1 and "NULL" in lib.goenv_last_error().decode()
+
+
+def test_nothing_to_copy_is_no_error(lib):
+    for change in (dict(rows=0, legal=256), dict(cols=0, legal=256), dict(legal=256, history=256, history_max=0)):
+        args = (256 if "rows" in change or "cols" in change else None, 256 if "history" in change else None, None)
+        assert lib.goenv_policy_logits_keep(C.byref(rules(**change)), *args, None) == 0
