@@ -50,9 +50,15 @@ int dtype_of(at::ScalarType t) { return t == at::kFloat ? GOENV_DT_F32 : t == at
 
 // ---- arguments ------------------------------------------------------------------------------------
 
+// What a kernel, which sees memory and no more, would lose
+void check_plain(const Tensor& t, const char* name) {
+  if (t._fw_grad(/*level=*/0).defined()) refuse(name, " carries a forward-mode derivative: the policy-network operators have none");
+}
+
 Tensor main_tensor(py::handle h, const char* name) {
   if (!THPVariable_Check(h.ptr())) refuse(name, " must be a tensor on the GPU");
   const Tensor& t = THPVariable_Unpack(h.ptr());
+  check_plain(t, name);
   if (!t.is_cuda() || t.layout() != at::kStrided) refuse(name, " must be a tensor on the GPU");
   if (!is_float_type(t.scalar_type())) refuse(name, " must be float32, bfloat16 or float16 (got ", t.scalar_type(), ")");
   return t.resolve_neg();   // (the imaginary part of a conjugate: its memory holds the values with the other sign)
@@ -61,7 +67,9 @@ Tensor main_tensor(py::handle h, const char* name) {
 Tensor optional_tensor(py::handle h, const char* name) {
   if (h.is_none()) return Tensor();
   if (!THPVariable_Check(h.ptr())) refuse(name, " must be a tensor (got ", py::str(py::type::handle_of(h)).cast<std::string>(), ")");
-  return THPVariable_Unpack(h.ptr()).resolve_neg();
+  const Tensor& t = THPVariable_Unpack(h.ptr());
+  check_plain(t, name);
+  return t.resolve_neg();
 }
 
 void check_like(const Tensor& t, const char* name, const Tensor& like, std::initializer_list<at::ScalarType> types, at::IntArrayRef shape) {
@@ -242,6 +250,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain(grads[0], "the gradient");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &bias = saved[3];
     const NormHow how{ctx->saved_data["groups"].toInt(), (float)ctx->saved_data["eps"].toDouble(), (float)ctx->saved_data["slope"].toDouble(),
@@ -352,6 +361,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     return dropout_run(x, residual, how.p, how.rng, how.site);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain(grads[0], "the gradient");
     const Tensor rng = ctx->get_saved_variables()[0];
     variable_list out(3);
     if (ctx->needs_input_grad(0)) {
@@ -500,6 +510,7 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain(grads[0], "the gradient");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &bias = saved[1], &copy = saved[3];
     LogitHow how{{}, {}, {}, {}, {saved[4], saved[5], saved[6], saved[7]}, {}, (int)ctx->saved_data["kind"].toInt(),

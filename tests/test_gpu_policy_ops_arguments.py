@@ -108,3 +108,31 @@ def test_copies_of_rules(ops, rows, cols, start, stride, moves):
             assert torch.equal(bits[:own * words].view(own, words), bits_of[:own]) and bool((bits[own * words:] == 77).all())
             assert torch.equal(moved[:own * moves].view(own, moves), h[:own]) and bool((moved[own * moves:] == 78).all())
             assert torch.equal(lens[:rows], many) and bool((lens[rows:] == 79).all())
+
+
+def test_forward_mode_derivatives_are_refused(ops, error):
+    """A tangent would be lost: the operators have no forward-mode derivatives.  Outside a dual level, or with a primal alone, nothing is."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w, l = randn(5, 2, 9, 8).transpose(1, 2), randn(6, 8), randn(7, 3, 40)
+    rng, t = torch.tensor([1, 2], device="cuda"), torch.ones(3, device="cuda")
+    want = ops.group_norm_act(x, 2, w), ops.dropout(x, 0.5, rng), ops.policy_logits(l, out="probs")
+    leaf, row = x.clone(memory_format=torch.preserve_format).requires_grad_(True), l.clone().requires_grad_(True)
+    with forward_ad.dual_level():
+        dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))                     # noqa: E731
+        calls = [lambda: ops.group_norm_act(dual(x), 2), lambda: ops.group_norm_act(x, 2, dual(w)), lambda: ops.group_norm_act(x, 2, w, dual(w)),
+                 lambda: ops.group_norm_act(x, 2, residual=dual(x)), lambda: ops.dropout(dual(x), 0.5, rng),
+                 lambda: ops.dropout(x, 0.5, rng, residual=dual(x)), lambda: ops.policy_logits(dual(l)),
+                 lambda: ops.policy_logits(l, bias=dual(randn(8, 40))), lambda: ops.policy_logits(l, temperature=dual(t)),
+                 lambda: ops.group_norm_act(dual(x.clone(memory_format=torch.preserve_format).requires_grad_(True)), 2)]
+        for call in calls:
+            with pytest.raises(error, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(error, match="forward-mode"):
+                call()
+        assert torch.equal(ops.group_norm_act(x, 2, w), want[0]) and torch.equal(ops.dropout(x, 0.5, rng), want[1])
+        for y, v in ((ops.group_norm_act(leaf, 2, w), leaf), (ops.dropout(leaf, 0.5, rng), leaf), (ops.policy_logits(row, out="probs"), row)):
+            with pytest.raises(RuntimeError, match="forward-mode"):                      # in the backward pass
+                torch.autograd.grad(y, v, dual(torch.ones_like(y)))
+        primal = forward_ad.unpack_dual(dual(l)).primal
+        assert torch.equal(ops.policy_logits(primal, out="probs"), want[2])
+    assert torch.equal(ops.policy_logits(l, out="probs"), want[2])

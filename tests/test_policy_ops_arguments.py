@@ -2,6 +2,7 @@
 import ctypes as C
 
 import pytest
+import torch
 
 
 @pytest.fixture(scope="module")
@@ -35,3 +36,23 @@ def test_nothing_to_copy_is_no_error(lib):
     for change in (dict(rows=0, legal=256), dict(cols=0, legal=256), dict(legal=256, history=256, history_max=0)):
         args = (256 if "rows" in change or "cols" in change else None, 256 if "history" in change else None, None)
         assert lib.goenv_policy_logits_keep(C.byref(rules(**change)), *args, None) == 0
+
+
+def operators():
+    """{name: call of (tensor)} of arguments that pass every check but that of the device."""
+    from elf_amd import policy_ops
+    rng = torch.zeros(2, dtype=torch.int64)
+    return {"group_norm_act": lambda x: policy_ops.group_norm_act(x.t(), 2), "dropout": lambda x: policy_ops.dropout(x, 0.5, rng),
+            "policy_logits": lambda x: policy_ops.policy_logits(x)}
+
+
+@pytest.mark.parametrize("name", ["group_norm_act", "dropout", "policy_logits"])
+def test_forward_mode_derivatives_are_refused(name):
+    import torch.autograd.forward_ad as forward_ad
+    from elf_amd import goenv
+    call, x = operators()[name], torch.ones(8, 6)
+    with forward_ad.dual_level():
+        with pytest.raises(goenv.GoEnvError, match="forward-mode"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(goenv.GoEnvError, match="on the GPU"):
+            call(x)
