@@ -3,6 +3,7 @@
 // In C++ because the backward pass of a small tensor costs more in Python (the engine's thread has to take the interpreter's
 // lock) than its kernels take: a dropout of 255 x 722, forward and backward, took 97 us there and 46 here.  Every kernel is reached through the C-ABI.
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -10,6 +11,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -53,6 +55,14 @@ int dtype_of(at::ScalarType t) { return t == at::kFloat ? GOENV_DT_F32 : t == at
 // What a kernel, which sees memory and no more, would lose
 void check_plain(const Tensor& t, const char* name) {
   if (t._fw_grad(/*level=*/0).defined()) refuse(name, " carries a forward-mode derivative: the policy-network operators have none");
+}
+
+// A trace would record the outputs' allocation and not what fills them
+void check_not_traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE))
+    refuse("the policy-network operators cannot be recorded in a trace");
 }
 
 Tensor main_tensor(py::handle h, const char* name) {
@@ -283,6 +293,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 
 Tensor group_norm_act(py::handle px, py::handle pgroups, py::handle pweight, py::handle pbias, py::handle peps, const std::string& act, py::handle pslope,
                       py::handle presidual) {
+  check_not_traced();
   const Tensor x = main_tensor(px, "x");
   if (x.dim() < 2) refuse("x must be [n, c, *positions] (got ", x.sizes(), ")");
   if (!layout_of(x).ok)
@@ -378,6 +389,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
 };
 
 Tensor dropout(py::handle px, py::handle pp, py::handle prng, py::handle psite, py::handle presidual) {
+  check_not_traced();
   const Tensor x = main_tensor(px, "x");
   if (!is_dense(x)) refuse("x must be dense (contiguous or channels last); got shape ", x.sizes(), ", strides ", x.strides());
   const double p = number(pp, "p must be a number from 0 to 1: it");
@@ -541,6 +553,7 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
 
 Tensor policy_logits(py::handle plogits, py::handle plegal, py::handle pbits, py::handle pbias, py::handle phistory, py::handle plen, py::handle prepetition,
                      py::handle ppresence, py::handle pfrequency, py::handle ptemperature, const std::string& out, py::handle pdtype) {
+  check_not_traced();
   const Tensor logits = main_tensor(plogits, "logits");
   if (logits.dim() != 2) refuse("logits must be [rows, cols] (got ", logits.sizes(), ")");
   const int64_t rows = logits.size(0), cols = logits.size(1);

@@ -9,7 +9,7 @@ All of them take torch-ROCm tensors, run on torch's current stream of the tensor
 nothing that outlives the call) through torch, and can be captured into a graph.  (A backward pass under capture needs leaves
 no eager graph of which lives on the default stream; a call under capture with such a leaf is refused.)  What they refuse raises
 :class:`elf_amd.goenv.GoEnvError`.  Gradients: once, through the backward pass of ``torch.autograd``; a tensor with a forward-mode derivative is
-refused.  There is no CPU fallback.
+refused, and so is a call while torch records a trace (``torch.jit.trace``, ``make_fx``).  There is no CPU fallback.
 """
 import torch
 import torch.nn as nn

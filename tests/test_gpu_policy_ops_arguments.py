@@ -136,3 +136,16 @@ def test_forward_mode_derivatives_are_refused(ops, error):
         primal = forward_ad.unpack_dual(dual(l)).primal
         assert torch.equal(ops.policy_logits(primal, out="probs"), want[2])
     assert torch.equal(ops.policy_logits(l, out="probs"), want[2])
+
+
+def test_calls_under_a_trace_are_refused(ops, error):
+    """A trace records the allocation of an output and not what fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, l, rng = randn(9, 2, 9, 8).transpose(1, 2), randn(10, 3, 40), torch.tensor([1, 2], device="cuda")
+    for f, v in ((lambda x: ops.group_norm_act(x, 2) + x, x), (lambda x: ops.dropout(x, 0.5, rng) + x, x), (lambda v: ops.policy_logits(v) + v, l)):
+        with pytest.raises(error, match="trace"):
+            torch.jit.trace(f, (v,), check_trace=False)
+        for mode in ("real", "fake"):
+            with pytest.raises(error, match="trace"):
+                make_fx(f, tracing_mode=mode)(v)
+        assert torch.equal(f(v), f(v))

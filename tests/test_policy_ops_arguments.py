@@ -56,3 +56,17 @@ def test_forward_mode_derivatives_are_refused(name):
             call(forward_ad.make_dual(x, torch.ones_like(x)))
         with pytest.raises(goenv.GoEnvError, match="on the GPU"):
             call(x)
+
+
+@pytest.mark.parametrize("name", ["group_norm_act", "dropout", "policy_logits"])
+def test_calls_under_a_trace_are_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from elf_amd import goenv
+    call, x = operators()[name], torch.ones(8, 6)
+    with pytest.raises(goenv.GoEnvError, match="trace"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    for mode in ("real", "fake"):
+        with pytest.raises(goenv.GoEnvError, match="trace"):
+            make_fx(call, tracing_mode=mode)(x)
+    with pytest.raises(goenv.GoEnvError, match="on the GPU"):
+        call(x)
