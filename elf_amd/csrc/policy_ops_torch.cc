@@ -55,6 +55,9 @@ int dtype_of(at::ScalarType t) { return t == at::kFloat ? GOENV_DT_F32 : t == at
 // What a kernel, which sees memory and no more, would lose
 void check_plain(const Tensor& t, const char* name) {
   if (t._fw_grad(/*level=*/0).defined()) refuse(name, " carries a forward-mode derivative: the policy-network operators have none");
+  // (to a kernel an optional argument without memory is one that was left out)
+  if (t.layout() == at::kStrided && (!t.has_storage() || (t.numel() > 0 && t.const_data_ptr() == nullptr)))
+    refuse(name, " must have memory of its own (a plain tensor, not a wrapper or a placeholder of one)");
 }
 
 // A trace would record the outputs' allocation and not what fills them

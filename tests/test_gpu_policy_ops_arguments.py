@@ -149,3 +149,29 @@ def test_calls_under_a_trace_are_refused(ops, error):
             with pytest.raises(error, match="trace"):
                 make_fx(f, tracing_mode=mode)(v)
         assert torch.equal(f(v), f(v))
+
+
+def test_tensors_without_memory_are_refused(ops, error):
+    """Some tensors have a type, a device and sizes but no memory (torch's lazy zeros, wrappers of other tensors): as an optional
+    argument one would count as left out."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.size(), strides=t.stride(), dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(func)
+    x, w, l = randn(11, 2, 9, 8).transpose(1, 2), randn(12, 8), randn(13, 3, 40)
+    rng, legal, past = torch.tensor([1, 2], device="cuda"), torch.zeros(3, 40, dtype=torch.uint8, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    for other in (Wrapper, lambda t: torch._efficientzerotensor(t.shape, dtype=t.dtype, device=t.device)):
+        for call in (lambda: ops.group_norm_act(x, 2, other(w)), lambda: ops.group_norm_act(x, 2, w, other(w)), lambda: ops.dropout(x, 0.5, other(rng)),
+                     lambda: ops.policy_logits(l, legal=other(legal)), lambda: ops.policy_logits(l, bias=other(l[0])),
+                     lambda: ops.policy_logits(l, history=other(past)), lambda: ops.policy_logits(l, temperature=other(l[:, 0]))):
+            with pytest.raises(error, match="memory"):
+                call()
+    for call in (lambda: ops.group_norm_act(x, 2, residual=Wrapper(x)), lambda: ops.dropout(x, 0.5, rng, residual=Wrapper(x)),
+                 lambda: ops.group_norm_act(Wrapper(x), 2), lambda: ops.policy_logits(Wrapper(l))):
+        with pytest.raises(error, match="memory"):
+            call()
+    assert torch.equal(ops.policy_logits(l, history=past[:, :0]), l)                     # nothing to hold, nothing missing

@@ -70,3 +70,26 @@ def test_calls_under_a_trace_are_refused(name):
             make_fx(call, tracing_mode=mode)(x)
     with pytest.raises(goenv.GoEnvError, match="on the GPU"):
         call(x)
+
+
+class Wrapper(torch.Tensor):
+    """A tensor with a type and sizes that holds another one and no memory of its own."""
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.size(), strides=t.stride(), dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(func)
+
+
+def test_tensors_without_memory_are_refused():
+    from elf_amd import goenv, policy_ops
+    x = torch.ones(6, 8)
+    for other in (Wrapper(x), torch._efficientzerotensor(6, 8)):
+        for call in (lambda t: policy_ops.group_norm_act(t, 2), lambda t: policy_ops.dropout(t, 0.5, torch.zeros(2, dtype=torch.int64)),
+                     policy_ops.policy_logits):
+            with pytest.raises(goenv.GoEnvError, match="memory"):
+                call(other)
+    with pytest.raises(goenv.GoEnvError, match="on the GPU"):
+        policy_ops.group_norm_act(x[:0], 2)
