@@ -556,6 +556,8 @@ struct LogitPlan {
   int threads, vec, ni;
   bool split, wave;   // wave: a wave a slice, four a workgroup
   unsigned blocks(int64_t teams) const { return (unsigned)(wave ? (teams + 3) / 4 : teams); }
+  // Of a launch, whose threads are to stay below 2^31; more rows take several, one after the other (and the workspace in turn)
+  int64_t rows_at_once() const { return (int64_t)(INT32_MAX / threads) * (wave ? 4 : 1) / cut.slices; }
 };
 
 // The cut for vectors of `vec` columns (which goes by the arrays' alignment: a workspace is sized for either).
@@ -585,6 +587,29 @@ LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, int 
   }
   p.cut.groups = (rows + p.cut.per_group - 1) / p.cut.per_group;
   return p;
+}
+
+int64_t size_of(int dt) { return dt == GOENV_DT_F32 ? 4 : 2; }
+template <typename P>
+P* past(P* p, int64_t bytes) {   // (no array stays none)
+  return p ? reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + bytes) : nullptr;
+}
+// The rules of `rows` rows from `first` on
+goenv_logit_rules rules_from(const goenv_logit_rules& p, int64_t first, int64_t rows) {
+  goenv_logit_rules q = p;
+  q.rows = rows;
+  q.logits = past(p.logits, first * p.logits_row * size_of(p.dtype));
+  q.legal = past(p.legal, first * p.legal_row);
+  q.legal_bits = past(p.legal_bits, first * p.bits_row * 4);
+  q.bias = past(p.bias, first * p.bias_row * size_of(p.bias_dtype));
+  q.history = past(p.history, first * p.history_row * (p.history_i64 ? 8 : 4));
+  q.history_len = past(p.history_len, first * 4);
+  q.row_repetition = past(p.row_repetition, first * 4);
+  q.row_presence = past(p.row_presence, first * 4);
+  q.row_frequency = past(p.row_frequency, first * 4);
+  q.row_temperature = past(p.row_temperature, first * 4);
+  q.stats = past(p.stats, first * 8);
+  return q;
 }
 
 // Whether all arrays allow vectors of four columns
@@ -679,30 +704,33 @@ int goenv_policy_logits(const goenv_logit_rules* p, void* out, void* stream) {
   if (!out || !aligned(out, p->out_dtype)) return fail("goenv_policy_logits: out is required, aligned to its elements");
   const bool softmax = p->out_kind != GOENV_OUT_LOGITS;
   const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, false, logit_fours(p, nullptr, 0, out, p->out_dtype, nullptr, 0) ? 4 : 1);
-  if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits");
-  by_dtype(p->dtype, [&](auto t) {
-    using T = decltype(t);
-    auto with = [&](auto v, auto n) {
-      constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
-      const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
-      auto go = [&](auto f) {
-        hipLaunchKernelGGL(f, dim3(plan.blocks(p->rows * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, out);
+  for (int64_t first = 0, each = plan.rows_at_once(); first < p->rows; first += each) {
+    const goenv_logit_rules q = rules_from(*p, first, each < p->rows - first ? each : p->rows - first);
+    void* to = past(out, first * p->cols * size_of(p->out_dtype));
+    by_dtype(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      auto with = [&](auto v, auto n) {
+        constexpr int VEC = decltype(v)::value, NI = decltype(n)::value;
+        const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
+        auto go = [&](auto f) {
+          hipLaunchKernelGGL(f, dim3(plan.blocks(q.rows * plan.cut.slices)), dim3(plan.threads), lds, S(stream), q, plan.cut, to);
+        };
+        if constexpr (VEC == 1 && NI == 12) {
+          go(k_policy_logits<T, VEC, NI, false, LOGIT_WHOLE>);
+        } else if (!softmax) {
+          plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_MAP>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_MAP>);
+        } else if (!plan.split) {
+          plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_WHOLE>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_WHOLE>);
+        } else {
+          go(k_policy_logits<T, VEC, NI, false, LOGIT_SUMS>);
+          go(k_policy_logits<T, VEC, NI, false, LOGIT_APPLY>);
+        }
       };
-      if constexpr (VEC == 1 && NI == 12) {
-        go(k_policy_logits<T, VEC, NI, false, LOGIT_WHOLE>);
-      } else if (!softmax) {
-        plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_MAP>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_MAP>);
-      } else if (!plan.split) {
-        plan.wave ? go(k_policy_logits<T, VEC, NI, true, LOGIT_WHOLE>) : go(k_policy_logits<T, VEC, NI, false, LOGIT_WHOLE>);
-      } else {
-        go(k_policy_logits<T, VEC, NI, false, LOGIT_SUMS>);
-        go(k_policy_logits<T, VEC, NI, false, LOGIT_APPLY>);
-      }
-    };
-    plan.vec == 4 ? with(Int<4>(), Int<4>()) : plan.ni == 12 ? with(Int<1>(), Int<12>()) : with(Int<1>(), Int<6>());
-  });
-  HIPCHK(hipGetLastError());
+      plan.vec == 4 ? with(Int<4>(), Int<4>()) : plan.ni == 12 ? with(Int<1>(), Int<12>()) : with(Int<1>(), Int<6>());
+    });
+    HIPCHK(hipGetLastError());
+  }
   return 0;
 }
 
@@ -715,11 +743,17 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
     return fail("goenv_policy_logits_grad: d_out is required, and the arrays aligned to their elements");
   const LogitPlan plan = logit_plan(p->rows, p->cols, softmax, shared,
                                     logit_fours(p, d_out, dy_row, dlogits, p->dtype, shared ? nullptr : dbias, p->bias_dtype) ? 4 : 1);
-  if (p->rows * plan.cut.slices > INT32_MAX / plan.threads) return fail("goenv_policy_logits_grad: too many rows for one launch");
   ON_DEVICE(p->device, "goenv_policy_logits_grad");
   const int64_t sums = plan.split ? (p->rows * plan.cut.slices * (int64_t)sizeof(float) + 15) & ~15 : 0;
   float* parts = shared ? reinterpret_cast<float*>(static_cast<char*>(p->workspace) + sums) : nullptr;
-  if (p->rows > 0) {
+  // (the gradient of a shared bias takes all rows in one launch: a workgroup has as many as it takes)
+  for (int64_t first = 0, each = shared ? p->rows : plan.rows_at_once(); first < p->rows; first += each) {
+    const goenv_logit_rules q = rules_from(*p, first, each < p->rows - first ? each : p->rows - first);
+    LogitCut cut = plan.cut;
+    if (!shared) cut.groups = q.rows;
+    const void* dy = past(d_out, first * dy_row * size_of(p->out_dtype));
+    void* dl = past(dlogits, first * p->cols * size_of(p->dtype));
+    void* db = past(dbias, first * p->cols * size_of(p->bias_dtype));
     by_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
       auto with = [&](auto v, auto n, auto b) {
@@ -727,8 +761,8 @@ int goenv_policy_logits_grad(const goenv_logit_rules* p, const void* d_out, int6
         constexpr bool SHARED = decltype(b)::value;
         const size_t lds = p->history ? (size_t)plan.threads * VEC * NI * sizeof(int) : 0;
         auto go = [&](auto f) {
-          hipLaunchKernelGGL(f, dim3(plan.blocks(plan.cut.groups * plan.cut.slices)), dim3(plan.threads), lds, S(stream), *p, plan.cut, d_out,
-                             dy_row, static_cast<T*>(dlogits), dbias, parts);
+          hipLaunchKernelGGL(f, dim3(plan.blocks(cut.groups * cut.slices)), dim3(plan.threads), lds, S(stream), q, cut, dy, dy_row,
+                             static_cast<T*>(dl), db, parts);
         };
         auto launch = [&](auto w) {
           constexpr bool WAVE = decltype(w)::value;

@@ -175,3 +175,54 @@ def test_tensors_without_memory_are_refused(ops, error):
         with pytest.raises(error, match="memory"):
             call()
     assert torch.equal(ops.policy_logits(l, history=past[:, :0]), l)                     # nothing to hold, nothing missing
+
+
+@pytest.mark.parametrize("rows,cols,out,shared", [(9_000_001, 2, "probs", False), (8_500_000, 3, "log_probs", True), (34_000_003, 1, "logits", False)])
+def test_more_rows_than_a_launch(ops, rows, cols, out, shared):
+    """The first rows, the last ones and those in between, forward and backward, against the definition; a shared bias's gradient
+    against sums in 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    logits = torch.randn(rows, cols, device="cuda", generator=g).to(BF16)
+    legal = torch.rand(rows, cols, device="cuda", generator=g) < 0.7
+    past = torch.randint(-1, cols, (rows, 1), device="cuda", generator=g, dtype=torch.int32)
+    many = torch.randint(0, 2, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    t = 0.5 + torch.rand(rows, device="cuda", generator=g)
+    bias = torch.randn(*((cols,) if shared else (rows, cols)), device="cuda", generator=g)
+    dy = torch.randn(rows, cols, device="cuda", generator=g)
+    x, b = logits.requires_grad_(True), bias.requires_grad_(True)
+    y = ops.policy_logits(x, legal=legal, bias=b, history=past, history_len=many, presence=t, temperature=t, out=out, dtype=F32)
+    dx, db = torch.autograd.grad(y, (x, b), dy)
+    at = torch.cat([torch.arange(0, 40), torch.arange(1, 60) * (rows // 64), torch.arange((1 << 23) - 20, (1 << 23) + 20), torch.arange(rows - 40, rows)])
+    at = at[at < rows].cuda()
+    want = ref.policy_logits(logits.detach()[at], legal[at], bias.detach() if shared else bias.detach()[at], past[at], many[at], 1.0, t[at], 0.0, t[at], out, F32, dy[at])
+    assert_within(y[at], want["y"], "y")
+    assert_within(dx[at], want["dlogits"], "dlogits")
+    if not shared:
+        assert_within(db[at], want["dbias"], "dbias")
+        return
+    # every row's dz by torch, in 64 bits: dy - softmax(z) sum dy over the live columns, over t
+    z = ((logits.detach().double() - torch.where((past >= 0) & (many[:, None] > 0) & (past == torch.arange(cols, device="cuda")), t[:, None].double(), 0.0)
+          + bias.detach().double()) / t[:, None]).masked_fill(~legal, -float("inf"))
+    p = torch.softmax(z, 1).nan_to_num(0.0)
+    d = dy.double().masked_fill(~legal, 0.0)
+    dz = (d - p * d.sum(1, keepdim=True)) / t[:, None].double()
+    # a term is off by 60 roundings at most; a column's sum has rows / 64 + 128 roundings at most on the way of any term (64 threads or more share it)
+    bound = (60 + 128 + rows / 64) * ref.U * (dz.abs() + (p * d.sum(1, keepdim=True) / t[:, None]).abs() + (d / t[:, None]).abs()).sum(0)
+    assert bool(((db.double() - dz.sum(0)).abs() <= bound).all())
+
+
+def test_more_long_rows_than_a_launch(ops):
+    """Rows of several slices, which use the workspace, over more than one launch.  All rows are one row of logits; each third has a temperature
+    of its own, and equal rows give equal bits."""
+    rows, cols = 940_001, 13_001
+    x, dy = randn(15, 1, cols, dtype=BF16), randn(16, 1, cols, dtype=BF16)
+    t = torch.tensor([0.5, 1.0, 1.5], device="cuda").repeat(rows // 3 + 1)[:rows]
+    leaf = x[:1].expand(rows, cols).detach().requires_grad_(True)
+    y = ops.policy_logits(leaf, temperature=t, out="log_probs")
+    (dx,) = torch.autograd.grad(y, leaf, dy.expand(rows, cols))
+    want = ref.policy_logits(x.expand(3, cols), temperature=t[:3], out="log_probs", dy=dy.expand(3, cols))
+    assert_within(y[:3], want["y"], "y")
+    assert_within(dx[:3], want["dlogits"], "dlogits")
+    for all_rows in (y.detach(), dx):
+        for k in range(3):
+            assert bool((all_rows[k::3] == all_rows[k]).all())

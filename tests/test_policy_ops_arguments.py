@@ -93,3 +93,12 @@ def test_tensors_without_memory_are_refused():
                 call(other)
     with pytest.raises(goenv.GoEnvError, match="on the GPU"):
         policy_ops.group_norm_act(x[:0], 2)
+
+
+def test_no_number_of_rows_is_too_large_for_a_launch(lib):
+    """They reach the selection of the device (there is no such device: nothing is launched)."""
+    for change in (dict(rows=9_000_000, cols=2), dict(rows=1 << 33), dict(rows=1 << 20, cols=131072), dict(rows=3, cols=1 << 28)):
+        for bias in ({}, dict(bias=256, bias_row=0)):
+            p = rules(device=1 << 20, workspace=256, workspace_bytes=1 << 62, **change, **bias)
+            for rc in (lib.goenv_policy_logits(C.byref(p), 256, None), lib.goenv_policy_logits_grad(C.byref(p), 256, p.cols, 256, 256 if bias else None, None)):
+                assert rc == -1 and "selecting the device" in lib.goenv_last_error().decode()
