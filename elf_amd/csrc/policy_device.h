@@ -60,6 +60,12 @@ inline bool is_dtype(int dt) { return dt == GOENV_DT_F32 || dt == GOENV_DT_BF16 
 inline bool aligned(const void* p, int dt) { return ((uintptr_t)p & (dt == GOENV_DT_F32 ? 3 : 1)) == 0; }
 inline unsigned grid_of(int64_t items, int64_t most = 1 << 20) { return (unsigned)(items < most ? items : most); }
 
+// `bytes` on from p; no array stays none
+template <typename P>
+P* past(P* p, int64_t bytes) {
+  return p ? reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + bytes) : nullptr;
+}
+
 #define ON_DEVICE(dev, who)           \
   DeviceScope dev_scope_(dev);        \
   if (dev_scope_.err != hipSuccess) return fail(who ": selecting the device", dev_scope_.err)

@@ -821,6 +821,8 @@ struct NormPlan {
   int threads, vec;
   size_t lds;      // bytes of the staging launches
   bool split;
+  // Of a launch, whose threads are to stay below 2^31; more samples take several, one after the other
+  int64_t samples_at_once() const { return INT32_MAX / threads / cut.slabs / cut.chunks; }
 };
 
 // `vec` 0: the widest vector; else what the arrays' alignment allows (the cut into slabs and chunks stays the same)
@@ -1012,6 +1014,16 @@ int check_norm(const goenv_norm* p, bool grad) {
     return fail("goenv_group_norm_act: the workspace is too small or not 16-byte aligned (goenv_group_norm_workspace)");
   return 0;
 }
+// `n` samples from `first` on (their workspace apart)
+goenv_norm norm_from(const goenv_norm& p, int64_t first, int64_t n) {
+  const int64_t size = p.dtype == GOENV_DT_F32 ? 4 : 2;
+  goenv_norm q = p;
+  q.n = n;
+  q.x = past(p.x, first * p.x_sample * size);
+  q.residual = past(p.residual, first * p.r_sample * size);
+  q.stats = past(p.stats, first * p.groups * 8);
+  return q;
+}
 goenv_norm with_act(const goenv_norm* p) {
   goenv_norm q = *p;
   if (q.act == GOENV_ACT_LEAKY_RELU && q.slope == 0.f) q.act = GOENV_ACT_RELU;
@@ -1060,32 +1072,40 @@ int goenv_group_norm_act(const goenv_norm* p, void* y, void* stream) {
     return 0;
   }
   const NormPlan plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, false, norm_fit(&q, nullptr, 0, 0, y, nullptr));
-  if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks) return fail("goenv_group_norm_act: too many samples for one launch");
-  by_dtype(p->dtype, [&](auto t) {
-    using T = decltype(t);
-    if (plan.cut.rows == 0) {
+  if (plan.cut.rows == 0) {
+    by_dtype(p->dtype, [&](auto t) {
+      using T = decltype(t);
       hipLaunchKernelGGL((k_group_norm_any<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<T*>(y));
-      return;
-    }
-    by_vec<T>(plan.vec, [&](auto v) {
-      constexpr int VEC = decltype(v)::value;
-      const dim3 grid((unsigned)(q.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
-      const bool one = (q.channels / q.groups) % VEC == 0;
-      auto go = [&](auto f) { hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), q, plan.cut, static_cast<T*>(y)); };
-      auto with = [&](auto o, auto r) {
-        constexpr bool ONE = decltype(o)::value, RES = decltype(r)::value;
-        if (!plan.split) {
-          go(k_group_norm<T, VEC, ONE, RES, NORM_WHOLE>);
-        } else {
-          go(k_group_norm<T, VEC, ONE, false, NORM_SUMS>);
-          go(k_group_norm<T, VEC, ONE, RES, NORM_APPLY>);
-        }
-      };
-      if (one) q.residual ? with(Int<1>(), Int<1>()) : with(Int<1>(), Int<0>());
-      else q.residual ? with(Int<0>(), Int<1>()) : with(Int<0>(), Int<0>());
     });
-  });
-  HIPCHK(hipGetLastError());
+    HIPCHK(hipGetLastError());
+    return 0;
+  }
+  const int64_t each = plan.samples_at_once(), sample = q.positions * q.channels * (q.dtype == GOENV_DT_F32 ? 4 : 2);
+  if (each == 0) return fail("goenv_group_norm_act: too many groups for one launch");
+  for (int64_t first = 0; first < q.n; first += each) {
+    const goenv_norm part = norm_from(q, first, each < q.n - first ? each : q.n - first);
+    by_dtype(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      by_vec<T>(plan.vec, [&](auto v) {
+        constexpr int VEC = decltype(v)::value;
+        const dim3 grid((unsigned)(part.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
+        const bool one = (q.channels / q.groups) % VEC == 0;
+        auto go = [&](auto f) { hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), part, plan.cut, static_cast<T*>(past(y, first * sample))); };
+        auto with = [&](auto o, auto r) {
+          constexpr bool ONE = decltype(o)::value, RES = decltype(r)::value;
+          if (!plan.split) {
+            go(k_group_norm<T, VEC, ONE, RES, NORM_WHOLE>);
+          } else {
+            go(k_group_norm<T, VEC, ONE, false, NORM_SUMS>);
+            go(k_group_norm<T, VEC, ONE, RES, NORM_APPLY>);
+          }
+        };
+        if (one) q.residual ? with(Int<1>(), Int<1>()) : with(Int<1>(), Int<0>());
+        else q.residual ? with(Int<0>(), Int<1>()) : with(Int<0>(), Int<0>());
+      });
+    });
+    HIPCHK(hipGetLastError());
+  }
   return 0;
 }
 
@@ -1118,36 +1138,46 @@ int goenv_group_norm_act_grad(const goenv_norm* p, const void* dy, int64_t dy_sa
     HIPCHK(hipGetLastError());
   } else if (!empty) {
     plan = norm_plan(q.n, q.positions, q.channels, q.groups, q.dtype, q.residual != nullptr, true, norm_fit(&q, dy, dy_sample, dy_position, dx, dresidual));
-    if (q.n > INT32_MAX / plan.threads / plan.cut.slabs / plan.cut.chunks)
-      return fail("goenv_group_norm_act_grad: too many samples for one launch");
-    by_dtype(p->dtype, [&](auto t) {
-      using T = decltype(t);
-      if (plan.cut.rows == 0) {
-        plan.cut.chunks = 1;
+    if (plan.cut.rows == 0) {
+      plan.cut.chunks = 1;
+      by_dtype(p->dtype, [&](auto t) {
+        using T = decltype(t);
         hipLaunchKernelGGL((k_group_norm_any_grad<T>), dim3(grid_of(q.n * q.groups)), dim3(256), 0, S(stream), q, static_cast<const T*>(dy),
                            dy_sample, dy_position, static_cast<T*>(dx), static_cast<T*>(dresidual));
-        return;
-      }
-      by_vec<T>(plan.vec, [&](auto v) {
-        constexpr int VEC = decltype(v)::value;
-        const dim3 grid((unsigned)(q.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
-        auto go = [&](auto f) {
-          hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), q, plan.cut, static_cast<const T*>(dy), dy_sample, dy_position,
-                             static_cast<T*>(dx), static_cast<T*>(dresidual));
-        };
-        auto with = [&](auto r) {
-          constexpr bool RES = decltype(r)::value;
-          if (!plan.split) {
-            go(k_group_norm_grad<T, VEC, RES, NORM_WHOLE>);
-          } else {
-            go(k_group_norm_grad<T, VEC, RES, NORM_SUMS>);
-            if (dx || dresidual) go(k_group_norm_grad<T, VEC, RES, NORM_APPLY>);
-          }
-        };
-        q.residual ? with(Int<1>()) : with(Int<0>());
       });
-    });
-    HIPCHK(hipGetLastError());
+      HIPCHK(hipGetLastError());
+    } else {
+      const int64_t each = plan.samples_at_once(), size = q.dtype == GOENV_DT_F32 ? 4 : 2, sample = q.positions * q.channels * size;
+      if (each == 0) return fail("goenv_group_norm_act_grad: too many groups for one launch");
+      for (int64_t first = 0; first < q.n; first += each) {
+        goenv_norm part = norm_from(q, first, each < q.n - first ? each : q.n - first);
+        part.workspace = past(q.workspace, first * plan.cut.chunks * q.channels * (int64_t)sizeof(float2));
+        const void* g = past(dy, first * dy_sample * size);
+        void *gx = past(dx, first * sample), *gr = past(dresidual, first * sample);
+        by_dtype(p->dtype, [&](auto t) {
+          using T = decltype(t);
+          by_vec<T>(plan.vec, [&](auto v) {
+            constexpr int VEC = decltype(v)::value;
+            const dim3 grid((unsigned)(part.n * plan.cut.slabs * plan.cut.chunks)), block(plan.threads);
+            auto go = [&](auto f) {
+              hipLaunchKernelGGL(f, grid, block, plan.lds, S(stream), part, plan.cut, static_cast<const T*>(g), dy_sample, dy_position,
+                                 static_cast<T*>(gx), static_cast<T*>(gr));
+            };
+            auto with = [&](auto r) {
+              constexpr bool RES = decltype(r)::value;
+              if (!plan.split) {
+                go(k_group_norm_grad<T, VEC, RES, NORM_WHOLE>);
+              } else {
+                go(k_group_norm_grad<T, VEC, RES, NORM_SUMS>);
+                if (dx || dresidual) go(k_group_norm_grad<T, VEC, RES, NORM_APPLY>);
+              }
+            };
+            q.residual ? with(Int<1>()) : with(Int<0>());
+          });
+        });
+        HIPCHK(hipGetLastError());
+      }
+    }
   }
   if (dweight || dbias) {
     hipLaunchKernelGGL(k_group_norm_param_grad, dim3((q.channels + 15) / 16), dim3(1024), 0, S(stream),

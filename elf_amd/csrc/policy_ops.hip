@@ -590,10 +590,6 @@ LogitPlan logit_plan(int64_t rows, int64_t cols, bool softmax, bool shared, int 
 }
 
 int64_t size_of(int dt) { return dt == GOENV_DT_F32 ? 4 : 2; }
-template <typename P>
-P* past(P* p, int64_t bytes) {   // (no array stays none)
-  return p ? reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + bytes) : nullptr;
-}
 // The rules of `rows` rows from `first` on
 goenv_logit_rules rules_from(const goenv_logit_rules& p, int64_t first, int64_t rows) {
   goenv_logit_rules q = p;

@@ -226,3 +226,27 @@ def test_more_long_rows_than_a_launch(ops):
     for all_rows in (y.detach(), dx):
         for k in range(3):
             assert bool((all_rows[k::3] == all_rows[k]).all())
+
+
+def test_more_samples_than_a_launch(ops):
+    """34 million samples of nine values: more than 2^31 threads.  The last samples of each launch and of all, forward and backward."""
+    n = 34_000_003
+    x = torch.randn(n, 9, 1, device="cuda").to(F16).movedim(-1, 1).requires_grad_(True)
+    w, b = torch.full((1,), 1.25, device="cuda", requires_grad=True), torch.full((1,), 0.5, device="cuda", requires_grad=True)
+    y = ops.group_norm_act(x, 1, w, b, act="silu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), x.detach())
+    at = torch.cat([torch.arange(0, 20), torch.arange(1, 64) * (n // 64), torch.arange((1 << 25) - 70, (1 << 25) + 70), torch.arange(n - 20, n)]).cuda()
+    part = x.detach()[at]
+    want = ref.group_norm_act(part, 1, w, b, 1e-5, "silu", 0.1, None, part)
+    assert_within(y[at], want["y"], "y")
+    assert_within(dx[at], want["dx"], "dx")
+    v = x.detach().double()
+    xh = (v - v.mean(2, keepdim=True)) / torch.sqrt(v.var(2, keepdim=True, correction=0) + 1e-5)
+    z = xh * 1.25 + 0.5
+    s = torch.sigmoid(z)
+    dz = v * s * (1 + z * (1 - s))
+    # a term is off by 40 roundings of what it is made of (|dy|, |xh| below 8); 64 rows of n / 64 terms are added up one after the other, after a
+    # sample's own: n / 64 + 128 roundings at most on the way of any term
+    for got, terms in ((db, dz), (dw, dz * xh)):
+        bound = (n / 64 + 128) * ref.U * float(terms.abs().sum()) + 40 * ref.U * 8 * n * 9
+        assert abs(float(got) - float(terms.sum())) <= bound
