@@ -9,7 +9,7 @@ reference loads here.  Random-initialised when no checkpoint is given (none exis
 
 ``norm="group"`` puts group norm in place of BatchNorm: a position's outputs do not depend on the rest of its batch
 (selfplay batches of changing size, single positions), and norm, residual sum and activation are one kernel
-(``policy_ops.group_norm_act``; the net runs channels last).  ``dropout=p`` drops inside the residual blocks
+(``policy_ops.group_norm_act``; the net runs channels last; the heads, of two channels and one, have as many groups).  ``dropout=p`` drops inside the residual blocks
 while the net is in training mode (``policy_ops.dropout``; call ``next_step()`` after every optimizer step).
 """
 import math
@@ -26,6 +26,8 @@ class PolicyValueNet(nn.Module):
         super().__init__()
         if norm not in ("batch", "group"):
             raise ValueError("norm must be batch or group (got %r)" % (norm,))
+        if norm == "group" and (not isinstance(groups, int) or groups < 1 or dim % groups):
+            raise ValueError("groups must be a positive integer that divides the %d channels (got %r)" % (dim, groups))
         self.board_size, self.dim, self.num_block, self.bn = board_size, dim, num_block, bn
         self.groups = groups if norm == "group" else 0
         self.act = "leaky_relu" if leaky_relu else "relu"

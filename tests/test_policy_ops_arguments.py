@@ -102,3 +102,14 @@ def test_no_number_of_rows_is_too_large_for_a_launch(lib):
             p = rules(device=1 << 20, workspace=256, workspace_bytes=1 << 62, **change, **bias)
             for rc in (lib.goenv_policy_logits(C.byref(p), 256, None), lib.goenv_policy_logits_grad(C.byref(p), 256, p.cols, 256, 256 if bias else None, None)):
                 assert rc == -1 and "selecting the device" in lib.goenv_last_error().decode()
+
+
+@pytest.mark.parametrize("groups", [0, -8, 24, 256, 2.0])
+def test_a_net_of_groups_that_do_not_divide_its_channels_is_refused(groups):
+    """It would be a net of BatchNorm, or of another number of groups.  The heads (two channels and one) take what divides them."""
+    from elf_amd.df_model import PolicyValueNet
+    with pytest.raises(ValueError, match="groups"):
+        PolicyValueNet(dim=128, num_block=1, norm="group", groups=groups)
+    net = PolicyValueNet(dim=96, num_block=1, norm="group", groups=8)
+    assert [net.init_conv[1].num_groups, net.pi_final_conv[1].num_groups, net.value_final_conv[1].num_groups] == [8, 2, 1]
+    assert PolicyValueNet(dim=128, num_block=1, groups=groups).bn                         # not asked for: not looked at
