@@ -1007,7 +1007,7 @@ int check_norm(const goenv_norm* p, bool grad) {
   if (!p->x) return fail("goenv_group_norm_act: x is required");
   if (grad && !p->stats) return fail("goenv_group_norm_act_grad: the forward pass's stats are required");
   if (!aligned(p->x, p->dtype) || !aligned(p->residual, p->dtype) || !aligned(p->weight, p->param_dtype) ||
-      !aligned(p->bias, p->param_dtype))
+      !aligned(p->bias, p->param_dtype) || !aligned(p->stats, GOENV_DT_F32))
     return fail("goenv_group_norm_act: an array is not aligned to its elements");
   const int64_t need = goenv_group_norm_workspace(p->n, p->positions, p->channels, p->groups, p->dtype, grad);
   if (need > 0 && (!p->workspace || (int64_t)p->workspace_bytes < need || ((uintptr_t)p->workspace & 15)))

@@ -643,7 +643,9 @@ int check_logits(const goenv_logit_rules* p, bool grad) {
   if (!p->logits) return fail("goenv_policy_logits: logits is required");
   if (grad && p->out_kind != GOENV_OUT_LOGITS && !p->stats)
     return fail("goenv_policy_logits_grad: the forward pass's stats are required");
-  if (!aligned(p->logits, p->dtype) || !aligned(p->bias, p->bias_dtype) || ((uintptr_t)p->legal_bits & 3) ||
+  const uintptr_t words = (uintptr_t)p->legal_bits | (uintptr_t)p->history_len | (uintptr_t)p->stats | (uintptr_t)p->row_repetition |
+                          (uintptr_t)p->row_presence | (uintptr_t)p->row_frequency | (uintptr_t)p->row_temperature;
+  if (!aligned(p->logits, p->dtype) || !aligned(p->bias, p->bias_dtype) || (words & 3) ||
       ((uintptr_t)p->history & (p->history_i64 ? 7 : 3)))
     return fail("goenv_policy_logits: an array is not aligned to its elements");
   const int64_t need = goenv_policy_logits_workspace(p->rows, p->cols, p->out_kind, p->bias && p->bias_row == 0, grad);

@@ -113,3 +113,19 @@ def test_a_net_of_groups_that_do_not_divide_its_channels_is_refused(groups):
     net = PolicyValueNet(dim=96, num_block=1, norm="group", groups=8)
     assert [net.init_conv[1].num_groups, net.pi_final_conv[1].num_groups, net.value_final_conv[1].num_groups] == [8, 2, 1]
     assert PolicyValueNet(dim=128, num_block=1, groups=groups).bn                         # not asked for: not looked at
+
+
+@pytest.mark.parametrize("name", ["row_repetition", "row_presence", "row_frequency", "row_temperature", "stats", "history_len"])
+def test_rows_that_are_not_aligned_are_refused(lib, name):
+    """A scalar load drops the low bits of an address: it would be another row's value."""
+    p = rules(device=1 << 20, history=256, history_max=4, workspace=256, workspace_bytes=1 << 40, **{name: 258})
+    for rc in (lib.goenv_policy_logits(C.byref(p), 256, None), lib.goenv_policy_logits_grad(C.byref(p), 256, 361, 256, None, None)):
+        assert rc == -1 and "aligned" in lib.goenv_last_error().decode()
+
+
+def test_statistics_that_are_not_aligned_are_refused(lib):
+    from elf_amd import goenv
+    p = goenv.Norm(device=1 << 20, dtype=1, param_dtype=0, act=0, n=2, positions=9, channels=8, groups=2, eps=1e-5, x=256, x_sample=72, x_position=8,
+                   stats=258, workspace=256, workspace_bytes=1 << 40)
+    for rc in (lib.goenv_group_norm_act(C.byref(p), 256, None), lib.goenv_group_norm_act_grad(C.byref(p), 256, 72, 8, 256, None, None, None, None)):
+        assert rc == -1 and "aligned" in lib.goenv_last_error().decode()
