@@ -250,3 +250,58 @@ def test_more_samples_than_a_launch(ops):
     for got, terms in ((db, dz), (dw, dz * xh)):
         bound = (n / 64 + 128) * ref.U * float(terms.abs().sum()) + 40 * ref.U * 8 * n * 9
         assert abs(float(got) - float(terms.sum())) <= bound
+
+
+@pytest.mark.parametrize("cols", [361, 9000, 20001])
+@pytest.mark.parametrize("out", ["logits", "log_probs", "probs"])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_lowest_values_are_not_off(ops, cols, out, temperature):
+    """A column at the type's lowest value is live: its logit and log probability are finite, its probability is 0, and it passes its gradient on.  The
+    other columns are those of the row without it, within the bounds of that row."""
+    g = torch.Generator().manual_seed(17)
+    rows, lowest = 4, torch.finfo(F32).min
+    logits, dy = randn(18, rows, cols), randn(19, rows, cols)
+    legal = torch.rand(rows, cols, generator=g) < 0.7
+    low = torch.zeros(rows, cols, dtype=torch.bool)
+    low[:, 1::2] = True
+    low[3] = True                                    # a row with nothing else
+    bias = torch.where(low, lowest, 0.25).cuda()
+    kw = dict(history=torch.randint(0, cols, (rows, 30), generator=g).cuda(), repetition=1.5, presence=0.5, frequency=0.25, temperature=temperature, out=out)
+    x, b = logits.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    y = ops.policy_logits(x, legal=legal.cuda(), bias=b, **kw)
+    live, rest = legal & low, legal & ~low
+    rest[3] = False
+    y_cpu = y.detach().cpu()
+    assert torch.equal(y_cpu == -float("inf"), ~legal) if out != "probs" else bool((y_cpu[~legal] == 0).all())
+    # the row without its lowest values, in 64 bits
+    want = ref.policy_logits(logits, rest, torch.where(low, 0.0, 0.25).cuda(), dy=torch.where(low.cuda(), 0.0, dy), **kw)
+    value, bound = want["y"]
+    assert float(bound[:3].max()) < 1e-3             # (a bound that a wrong value would not meet)
+    assert bool(((y_cpu.double() - value).abs()[rest] <= bound[rest]).all())
+    if out == "probs":
+        assert not y_cpu[:3][live[:3]].any() and bool((y_cpu[rest & (value > 2 * ref.TINY)] > 0).all())
+    else:                                            # half a step of the sums and of the quotient, at this size
+        assert bool(((y_cpu.double() - lowest / temperature).abs()[:3][live[:3]] <= 8 * ref.U * -lowest).all())
+    # gradients: none from the lowest columns to the others
+    given = torch.where(low.cuda(), 0.0, dy)
+    given[3] = 0
+    dx, db = torch.autograd.grad(y, (x, b), given, retain_graph=True)
+    for d, k in ((dx, "dlogits"), (db, "dbias")):
+        value, bound = want[k]
+        assert float(bound[:3].max()) < 1e-3 and bool(((d.cpu().double() - value).abs()[:3] <= bound[:3]).all()), k
+    # their own: dy over the temperature where nothing else is given
+    only = torch.zeros(rows, cols, device="cuda")
+    only[:3, 1] = 3.0
+    (db,) = torch.autograd.grad(y, b, only)
+    own = 0.0 if out == "probs" else 3.0 / temperature
+    assert torch.equal(db[:3, 1].cpu(), torch.where(legal[:3, 1], own, 0.0))
+
+
+def test_a_row_of_lowest_values_is_even(ops):
+    """Every column as low as a number can be: a probability each like any other row of equals."""
+    for cols in (1, 361, 20001):
+        x = torch.full((2, cols), torch.finfo(F32).min, device="cuda")
+        p, logp = (ops.policy_logits(x, out=out).cpu().double() for out in ("probs", "log_probs"))
+        k = 24 + min(cols, 64 + cols // 64)          # roundings on the way of a term of the sum, and 8 of the quotient or the logarithm
+        assert float((p * cols - 1).abs().max()) <= (k + 8) * ref.U
+        assert float((logp + torch.tensor(float(cols)).double().log()).abs().max()) <= (k + 8) * ref.U * max(1.0, float(logp.abs().max()))
