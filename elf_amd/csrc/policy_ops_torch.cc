@@ -615,7 +615,7 @@ Tensor policy_logits(py::handle plogits, py::handle plegal, py::handle pbits, py
     const Tensor t = optional_tensor(given[i], names[i]);
     check_like(t, names[i], logits, {at::kFloat}, {rows});
     if (!t.is_contiguous()) refuse(names[i], " must be contiguous");
-    if (t.requires_grad()) refuse(names[i], " has no gradient (detach it)");
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(names[i], " has no gradient (detach it)");
     how.row[i] = t;
   }
   if (wants_grad({logits, bias})) return LogitNode::apply(logits, maybe(bias), how);

@@ -305,3 +305,15 @@ def test_a_row_of_lowest_values_is_even(ops):
         k = 24 + min(cols, 64 + cols // 64)          # roundings on the way of a term of the sum, and 8 of the quotient or the logarithm
         assert float((p * cols - 1).abs().max()) <= (k + 8) * ref.U
         assert float((logp + torch.tensor(float(cols)).double().log()).abs().max()) <= (k + 8) * ref.U * max(1.0, float(logp.abs().max()))
+
+
+def test_rules_with_a_gradient_where_none_is_wanted(ops, error):
+    """A learned temperature can be used where no gradients are taken; where they are, it is refused, since it would get none."""
+    l, t = randn(20, 3, 40), torch.full((3,), 0.5, device="cuda", requires_grad=True)
+    want = ops.policy_logits(l, temperature=0.5, out="probs")
+    with torch.no_grad():
+        assert torch.equal(ops.policy_logits(l, temperature=t, out="probs"), want)
+    with torch.inference_mode():
+        assert torch.equal(ops.policy_logits(l, temperature=t, out="probs"), want)
+    with pytest.raises(error, match="no gradient"):
+        ops.policy_logits(l, temperature=t)
