@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <cstring>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -420,7 +421,7 @@ struct LogitHow {
   at::ScalarType out_type;
 };
 
-goenv_logit_rules logit_args(const Tensor& logits, const Tensor& bias, const LogitHow& how, const Tensor& stats) {
+goenv_logit_rules logit_args(const Tensor& logits, const Tensor& bias, const LogitHow& how) {
   goenv_logit_rules p = {};
   p.device = logits.device().index();
   p.dtype = dtype_of(logits.scalar_type());
@@ -457,29 +458,30 @@ goenv_logit_rules logit_args(const Tensor& logits, const Tensor& bias, const Log
   const float** rows[4] = {&p.row_repetition, &p.row_presence, &p.row_frequency, &p.row_temperature};
   for (int i = 0; i < 4; ++i)
     if (how.row[i].defined()) *rows[i] = how.row[i].data_ptr<float>();
-  if (stats.defined()) p.stats = stats.data_ptr<float>();
   return p;
 }
 
-Tensor logits_forward(const Tensor& logits, const Tensor& bias, const LogitHow& how, const Tensor& stats) {
+Tensor logits_forward(const Tensor& logits, const LogitHow& how, goenv_logit_rules p) {
   Tensor out = at::empty(logits.sizes(), logits.options().dtype(how.out_type));
-  goenv_logit_rules p = logit_args(logits, bias, how, stats);
-  const int64_t need = goenv_policy_logits_workspace(p.rows, p.cols, p.out_kind, bias.defined() && p.bias_row == 0, 0);
+  const int64_t need = goenv_policy_logits_workspace(p.rows, p.cols, p.out_kind, 0, 0);
   const Tensor ws = workspace_of(need, logits);
   if (need > 0) p.workspace = ws.data_ptr(), p.workspace_bytes = need;
   check_rc(goenv_policy_logits(&p, out.data_ptr(), stream_of(logits)));
   return out;
 }
 
-// Copies of the mask (as bits), the histories and their lengths, one after the other in a tensor of bytes: the environment writes the next
-// position's into such buffers through plain pointers, of which a saved tensor's version count knows nothing.
+// What a node keeps in a tensor of bytes, one after the other: the rows' statistics, and copies of the histories, the mask (as bits) and the
+// histories' lengths -- the environment writes the next position's into such buffers through plain pointers, of which a saved
+// tensor's version count knows nothing.
 struct Kept {
-  int64_t mask_rows = 0, past_rows = 0, moves = 0, move_bytes = 0, lens = 0;
+  int64_t stats = 0, mask_rows = 0, past_rows = 0, moves = 0, move_bytes = 0, lens = 0;
   int64_t past_bytes() const { return past_rows * moves * move_bytes; }
-  int64_t bytes(int64_t words) const { return past_bytes() + (mask_rows * words + lens) * (int64_t)sizeof(int32_t); }
+  int64_t stats_bytes() const { return stats * 2 * (int64_t)sizeof(float); }
+  int64_t copy_bytes(int64_t words) const { return past_bytes() + (mask_rows * words + lens) * (int64_t)sizeof(int32_t); }
   static Kept of(const goenv_logit_rules& p) {   // (rows that are all the same one are kept once)
     Kept k;
     if (p.rows == 0 || p.cols == 0) return k;
+    if (p.out_kind != GOENV_OUT_LOGITS) k.stats = p.rows;
     if (p.legal || p.legal_bits) k.mask_rows = (p.legal ? p.legal_row : p.bits_row) == 0 ? 1 : p.rows;
     if (!p.history) return k;
     k.past_rows = p.history_row == 0 ? 1 : p.rows;
@@ -488,9 +490,11 @@ struct Kept {
     if (p.history_len) k.lens = p.rows;
     return k;
   }
-  // p with the copies that lie at `base`
+  // p with the statistics and copies that lie at `base`
   void to(goenv_logit_rules& p, char* base) const {
     const int64_t words = (p.cols + 31) / 32;
+    p.stats = stats ? reinterpret_cast<float*>(base) : nullptr;
+    base += stats_bytes();
     p.history = past_rows ? base : nullptr;
     p.history_row = past_rows == 1 ? 0 : moves;
     p.history_max = (int32_t)moves;
@@ -505,33 +509,39 @@ struct Kept {
 };
 
 struct LogitNode : torch::autograd::Function<LogitNode> {
+  struct Call {   // (a string in the node: one entry)
+    float scalar[4];
+    int out_kind;
+    at::ScalarType out_type;
+    Kept kept;
+  };
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Maybe& b, const LogitHow& how) {
     const Tensor bias = tensor_of(b);
-    const Tensor stats = how.out_kind == GOENV_OUT_LOGITS ? Tensor() : at::empty({logits.size(0), 2}, logits.options().dtype(at::kFloat));
-    Tensor out = logits_forward(logits, bias, how, stats), copy;
-    goenv_logit_rules p = logit_args(logits, Tensor(), how, Tensor()), own = p;
-    const Kept kept = Kept::of(p);
-    if (const int64_t bytes = kept.bytes((p.cols + 31) / 32)) {
-      copy = workspace_of(bytes, logits);
-      kept.to(own, static_cast<char*>(copy.data_ptr()));
+    goenv_logit_rules p = logit_args(logits, bias, how), own = p;
+    Call call{{}, how.out_kind, how.out_type, Kept::of(p)};
+    std::copy(how.scalar, how.scalar + 4, call.scalar);
+    const int64_t copies = call.kept.copy_bytes((p.cols + 31) / 32);
+    const Tensor memory = workspace_of(call.kept.stats_bytes() + copies, logits);
+    if (memory.defined()) {
+      call.kept.to(own, static_cast<char*>(memory.data_ptr()));
+      p.stats = own.stats;
+    }
+    Tensor out = logits_forward(logits, how, p);
+    if (copies > 0)
       check_rc(goenv_policy_logits_keep(&p, const_cast<uint32_t*>(own.legal_bits), const_cast<void*>(own.history), const_cast<int32_t*>(own.history_len),
                                         stream_of(logits)));
-    }
-    ctx->save_for_backward({logits, bias, stats, copy, how.row[0], how.row[1], how.row[2], how.row[3]});
-    ctx->saved_data["kept"] = std::vector<int64_t>{kept.mask_rows, kept.past_rows, kept.moves, kept.move_bytes, kept.lens};
-    ctx->saved_data["scalar"] = std::vector<double>(how.scalar, how.scalar + 4);
-    ctx->saved_data["kind"] = (int64_t)how.out_kind;
-    ctx->saved_data["type"] = (int64_t)how.out_type;
+    ctx->save_for_backward({logits, bias, memory, how.row[0], how.row[1], how.row[2], how.row[3]});
+    ctx->saved_data["call"] = std::string(reinterpret_cast<const char*>(&call), sizeof(call));
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_plain(grads[0], "the gradient");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &bias = saved[1], &copy = saved[3];
-    LogitHow how{{}, {}, {}, {}, {saved[4], saved[5], saved[6], saved[7]}, {}, (int)ctx->saved_data["kind"].toInt(),
-                 (at::ScalarType)ctx->saved_data["type"].toInt()};
-    const auto scalar = ctx->saved_data["scalar"].toDoubleVector();
-    for (int i = 0; i < 4; ++i) how.scalar[i] = (float)scalar[i];
+    const Tensor &logits = saved[0], &bias = saved[1], &memory = saved[2];
+    Call call;
+    std::memcpy(&call, ctx->saved_data["call"].toStringRef().data(), sizeof(call));
+    LogitHow how{{}, {}, {}, {}, {saved[3], saved[4], saved[5], saved[6]}, {}, call.out_kind, call.out_type};
+    std::copy(call.scalar, call.scalar + 4, how.scalar);
     variable_list out(3);
     {
       at::NoGradGuard no_grad;
@@ -540,9 +550,8 @@ struct LogitNode : torch::autograd::Function<LogitNode> {
       Needs needs{ctx};
       if (needs(logits)) out[0] = at::empty(logits.sizes(), logits.options());
       if (needs(bias)) out[1] = at::empty(bias.sizes(), bias.options());
-      goenv_logit_rules p = logit_args(logits, bias, how, saved[2]);
-      const auto kept = ctx->saved_data["kept"].toIntVector();
-      if (copy.defined()) Kept{kept[0], kept[1], kept[2], kept[3], kept[4]}.to(p, static_cast<char*>(copy.data_ptr()));
+      goenv_logit_rules p = logit_args(logits, bias, how);
+      if (memory.defined()) call.kept.to(p, static_cast<char*>(memory.data_ptr()));
       const int64_t need = goenv_policy_logits_workspace(p.rows, p.cols, p.out_kind, bias.defined() && p.bias_row == 0, 1);
       const Tensor ws = workspace_of(need, logits);
       if (need > 0) p.workspace = ws.data_ptr(), p.workspace_bytes = need;
@@ -619,7 +628,7 @@ Tensor policy_logits(py::handle plogits, py::handle plegal, py::handle pbits, py
     how.row[i] = t;
   }
   if (wants_grad({logits, bias})) return LogitNode::apply(logits, maybe(bias), how);
-  return logits_forward(logits, bias, how, Tensor());
+  return logits_forward(logits, how, logit_args(logits, bias, how));
 }
 
 }  // namespace
