@@ -79,9 +79,9 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t n, const T* x, const T*
 // A row's columns are cut into slices of threads x NI vectors of VEC columns, one workgroup each, with the slice's columns
 // in registers; how often a column stands in the row's history is counted in LDS (integers: the order does not matter).  Bound by
 // memory for many rows or long ones, by latency for a short one; so a row that fits one slice takes one launch and reads everything
-// once (8,192 rows of 361 bf16 columns with a mask and a history: 7.1 us, bound by instructions, some 285 a wave and row, since a row of
-// odd length has no vectors; 64 rows of 131,072 with histories of 2,048, no softmax: 36 MB, 10 us = 3.5 TB/s, bound by the
-// counts in LDS).  Longer rows take a launch for the slices' maxima and sums and one that joins them and computes z again, which costs
+// once (8,192 rows of 361 bf16 columns with a mask and a history: 7.1 us, bound by instructions, some 285 a wave and row, since a row
+// that is no multiple of four columns goes element by element; 64 rows of 131,072 with histories of 2,048, no softmax: 36 MB, 10.9 us =
+// 3.3 TB/s, where every slice scans the row's whole history).  Longer rows take a launch for the slices' maxima and sums and one that joins them and computes z again, which costs
 // reading the logits a second time (from the caches) instead of writing and reading z in 32 bits (one row of 131,072:
 // 4.3 and 4.1 us, of which a launch by itself takes 2).
 

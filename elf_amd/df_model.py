@@ -9,8 +9,9 @@ reference loads here.  Random-initialised when no checkpoint is given (none exis
 
 ``norm="group"`` puts group norm in place of BatchNorm: a position's outputs do not depend on the rest of its batch
 (selfplay batches of changing size, single positions), and norm, residual sum and activation are one kernel
-(``policy_ops.group_norm_act``; the net runs channels last; the heads, of two channels and one, have as many groups).  ``dropout=p`` drops inside the residual blocks
-while the net is in training mode (``policy_ops.dropout``; call ``next_step()`` after every optimizer step).
+(``policy_ops.group_norm_act``; the net runs channels last; ``groups`` divides ``dim``, and a head of two channels or one
+has gcd(groups, its channels)).  ``dropout=p`` drops inside the residual blocks while the net is in training mode
+(``policy_ops.dropout``; call ``next_step()`` after every optimizer step).
 """
 import math
 

@@ -35,7 +35,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
 
     x: [n, c, *positions], float32, bfloat16 or float16, channels last (``memory_format=torch.channels_last``, or any
     view whose channels lie next to each other: a slice of channels, of samples).  Statistics are taken per sample
-    over the positions and the c / num_groups channels of a group, in float32.  weight, bias: [c], float32 or x's
+    over the positions and the c / num_groups channels of a group, in float32.  (Groups of more than some 4,000 channels
+    are slow, above all their gradients.)  weight, bias: [c], float32 or x's
     type.  residual: of x's shape and type, channels last.  act: "none", "relu", "leaky_relu" (with `slope`) or
     "silu".  The result is dense and channels last, of x's type.  Gradients for x, residual, weight and bias."""
     return _ops().group_norm_act(x, num_groups, weight, bias, eps, act, slope, residual)
